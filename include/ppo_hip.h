@@ -312,6 +312,108 @@ int ppo_update_epochs(float* params, int state_dim, int action_dim, int continuo
                       double beta2, double eps, float* losses_out, void* workspace,
                       size_t workspace_bytes, void* stream);
 
+/* ---- policies over a large vocabulary -------------------------------------------------------------
+ * The same quantities for a policy whose action is one of `vocab` tokens and whose logits a model of the
+ * caller's has computed: log-probability and entropy (what ppo_evaluate gives for a small head), the clipped
+ * policy loss (ppo_epoch_fwdbwd's, with a KL term), a preference loss on pairs of sequences, and
+ * distillation from a teacher's top logits, each with its gradient with respect to the logits.  The
+ * reference has no counterpart: its Categorical head has a handful of actions (PPO.py:86-121).
+ *
+ * Rows: position t of sequence b of the logits is row r = b * n_tok + t, `vocab` consecutive elements at
+ * data + b * seq_stride + t * tok_stride (strides in elements; any values, also 0).  The gradient has the
+ * logits' type and strides of its own (no two rows may overlap); it may be the logits' own storage with the
+ * same strides, otherwise it must not overlap them.  Arrays "per row" are dense, in row order.
+ * mask (uint8 per row, NULL: all rows count): a row whose entry is 0 does not count.  Its logits, token and
+ * other inputs are not used in any way, its outputs are 0 and its row of the gradient is written as zeros.
+ * Logits of a counted row may hold -inf (an impossible token); +inf or NaN make its results NaN.  A token
+ * outside [0, vocab) of a counted row makes the row's results and its gradient NaN.
+ * Sums over the vocabulary and a row's scalars are fp32 and fp64; a gradient is rounded once, to nearest
+ * even, to the logits' type.  Results do not depend on other work on the GPU (no atomics).
+ * row_stats: 4 floats per row that the forward call leaves for its backward call.
+ * workspace: ppo_token_workspace_bytes(n_seq, n_tok) bytes, aligned to 16; calls that overlap in time (two
+ * streams, two captured graphs replayed together) need one each. */
+#define PPO_F32 0
+#define PPO_BF16 1
+#define PPO_F16 2
+#define PPO_MAX_VOCAB (1 << 30)
+#define PPO_MAX_TOKENS (1 << 30)       /* rows of one call */
+#define PPO_MAX_TEACHER_TOP 512
+
+#define PPO_REDUCE_SUM 0               /* weight of a counted row: scale */
+#define PPO_REDUCE_TOKEN_MEAN 1        /* scale / counted rows */
+#define PPO_REDUCE_SEQUENCE_MEAN 2     /* scale / (counted rows of its sequence * sequences that have one) */
+
+typedef struct {
+    const void* data;
+    int64_t seq_stride, tok_stride;           /* of the logits */
+    int64_t grad_seq_stride, grad_tok_stride; /* of the gradient, where one is written */
+    int64_t n_seq, n_tok, vocab;
+    int dtype;                                /* PPO_F32, PPO_BF16 or PPO_F16 */
+    float inv_temperature;                    /* probabilities are softmax(logits * inv_temperature) */
+} ppo_token_logits;
+
+size_t ppo_token_workspace_bytes(int64_t n_seq, int64_t n_tok);
+
+/* logprobs[r] of tokens[r] (int32, or int64 with tokens_are_i64) and, where entropy is not NULL, the
+ * entropy of the row's distribution.  row_stats may be NULL. */
+int ppo_token_logprobs(const ppo_token_logits* x, const void* tokens, int tokens_are_i64, const uint8_t* mask,
+                       float* logprobs, float* entropy, float* row_stats, void* stream);
+
+/* dL/dlogits from dL/dlogprob and dL/dentropy of each row (either may be NULL: zeros; each with a stride
+ * for sequences and one for tokens), both times *grad_factor (device; NULL: 1).  With grad_entropy the
+ * forward call must have computed the entropy. */
+int ppo_token_logprobs_backward(const ppo_token_logits* x, const void* tokens, int tokens_are_i64,
+                                const uint8_t* mask, const float* row_stats, const float* grad_logprobs,
+                                int64_t lp_seq_stride, int64_t lp_tok_stride, const float* grad_entropy,
+                                int64_t ent_seq_stride, int64_t ent_tok_stride, const float* grad_factor,
+                                void* grad, void* stream);
+
+/* Clipped policy loss: with ratio = exp(logprob - old) and d = ref - logprob of a row,
+ *   loss = sum over counted rows of weight * ( -min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A)
+ *                                              + kl_coef (exp(d) - d - 1) - entropy_coef H )
+ * (PPO.py:233-240 without the value term; the KL term is the estimator that is never negative).
+ * advantages has a stride for sequences and one for tokens (0: one for all); ref_logprobs may be NULL where
+ * kl_coef is 0.  loss: one float; logprobs, entropy (may be NULL): per row.
+ * grad != NULL: dloss/dlogits in the same pass over the logits.  Otherwise, with row_stats, the call leaves
+ * dloss/dlogprob and dloss/dentropy in seeds (2 floats per row: all of the first, then all of the second)
+ * for ppo_token_logprobs_backward. */
+typedef struct {
+    float clip_low, clip_high, kl_coef, entropy_coef, scale;
+    int reduction;
+} ppo_policy_terms;
+
+int ppo_policy_loss(const ppo_token_logits* x, const void* tokens, int tokens_are_i64, const uint8_t* mask,
+                    const float* old_logprobs, const float* advantages, int64_t adv_seq_stride,
+                    int64_t adv_tok_stride, const float* ref_logprobs, const ppo_policy_terms* terms,
+                    float* loss, float* logprobs, float* entropy, float* row_stats, float* seeds,
+                    void* grad, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Preference loss on n_seq / 2 pairs: sequence q is preferred to sequence q + n_seq / 2.
+ *   rewards[b] = beta (sum of the counted logprobs of sequence b - ref_logprobs[b]),  z = the pair's difference
+ *   loss = scale * mean over pairs of ( -(1 - label_smoothing) ln sigmoid(z) - label_smoothing ln sigmoid(-z) )
+ * A sequence without counted rows has the sum 0.  grad != NULL: dloss/dlogits too.  Otherwise, with
+ * row_stats, seeds (a float per sequence) receives dloss/dlogprob of each of its rows, for
+ * ppo_token_logprobs_backward with the strides (1, 0). */
+int ppo_preference_loss(const ppo_token_logits* x, const void* tokens, int tokens_are_i64, const uint8_t* mask,
+                        const float* ref_logprobs, double beta, double label_smoothing, double scale,
+                        float* loss, float* rewards, float* row_stats, float* seeds, void* grad,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* Distillation from a teacher's `top` best logits per row (teacher_tokens [rows, top], teacher_logits
+ * [rows, top] of a type of their own): q = softmax(teacher_logits * inv_temperature) over the entries whose
+ * token is not negative (others are padding), p the student's softmax over the whole vocabulary,
+ *   token_losses[r] = temperature^2 * sum_k q_k (ln q_k - ln p[token_k]),  loss = sum of weight * token_losses
+ * A row without entries has loss and gradient 0; a token that appears twice counts with both entries; a
+ * token >= vocab makes the row NaN.  top <= PPO_MAX_TEACHER_TOP.  grad != NULL: dloss/dlogits in the same
+ * pass; otherwise, with row_stats, ppo_distillation_backward computes it (times *grad_factor) later. */
+int ppo_distillation_loss(const ppo_token_logits* x, const void* teacher_tokens, int tokens_are_i64,
+                          const void* teacher_logits, int teacher_dtype, int top, const uint8_t* mask,
+                          int reduction, float scale, float* loss, float* token_losses, float* row_stats,
+                          void* grad, void* workspace, size_t workspace_bytes, void* stream);
+int ppo_distillation_backward(const ppo_token_logits* x, const void* teacher_tokens, int tokens_are_i64,
+                              const void* teacher_logits, int teacher_dtype, int top, const uint8_t* mask,
+                              const float* row_stats, const float* grad_factor, void* grad, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

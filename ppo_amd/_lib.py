@@ -11,7 +11,24 @@ import torch  # noqa: F401  (loads the HIP runtime the library binds to before d
 HERE = os.path.dirname(os.path.abspath(__file__))
 # PPO_HIP_LIB: diagnostic builds of the same sources (python -m ppo_amd.build --variant ...)
 LIB_PATH = os.environ.get("PPO_HIP_LIB") or os.path.join(HERE, "libppo_hip.so")
-ABI_VERSION = 10
+ABI_VERSION = 11
+
+
+class TokenLogits(ctypes.Structure):
+    """ppo_token_logits"""
+    _fields_ = [("data", c_void_p), ("seq_stride", c_int64), ("tok_stride", c_int64), ("grad_seq_stride", c_int64),
+                ("grad_tok_stride", c_int64), ("n_seq", c_int64), ("n_tok", c_int64), ("vocab", c_int64),
+                ("dtype", c_int), ("inv_temperature", c_float)]
+
+
+class PolicyTerms(ctypes.Structure):
+    """ppo_policy_terms"""
+    _fields_ = [("clip_low", c_float), ("clip_high", c_float), ("kl_coef", c_float), ("entropy_coef", c_float),
+                ("scale", c_float), ("reduction", c_int)]
+
+
+_LOGITS_P, _TERMS_P = ctypes.POINTER(TokenLogits), ctypes.POINTER(PolicyTerms)
+
 
 _SIGNATURES = {
     "ppo_hip_abi_version": (c_int, []),
@@ -72,6 +89,19 @@ _SIGNATURES = {
     "ppo_reduce_adam_step": (c_int, [c_int, c_int, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p,
                                      c_void_p, c_int64, c_double, c_double, c_double, c_double,
                                      c_double, c_void_p, c_void_p]),
+    "ppo_token_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "ppo_token_logprobs": (c_int, [_LOGITS_P, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "ppo_token_logprobs_backward": (c_int, [_LOGITS_P, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64,
+                                            c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "ppo_policy_loss": (c_int, [_LOGITS_P, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
+                                _TERMS_P, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                c_size_t, c_void_p]),
+    "ppo_preference_loss": (c_int, [_LOGITS_P, c_void_p, c_int, c_void_p, c_void_p, c_double, c_double, c_double,
+                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "ppo_distillation_loss": (c_int, [_LOGITS_P, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int, c_float,
+                                      c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "ppo_distillation_backward": (c_int, [_LOGITS_P, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p,
+                                          c_void_p, c_void_p, c_void_p]),
 }
 EXPORTS = tuple(_SIGNATURES)
 

@@ -15,11 +15,13 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libppo_hip.so")
 LIB_SYM = os.path.join(HERE, "libppo_hip_sym.so")
 FASTCALL = os.path.join(HERE, "_fastcall.so")          # CPython extension (csrc/fastcall.c), plain C
-SOURCES = ["scan.hip", "act.hip", "act_one.hip", "update.hip", "update_vjp.hip", "env.hip", "rollout.hip"]
+SOURCES = ["scan.hip", "act.hip", "act_one.hip", "update.hip", "update_vjp.hip", "env.hip", "rollout.hip", "token.hip"]
 SYM_SOURCES = ["update_sym.hip"]             # + update.hip compiled with -DPPO_WITH_SYM
 HEADERS = ["ppo_common.h", "update_common.h", os.path.join("..", "..", "include", "ppo_hip.h")]
 FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC",
          "-fhip-fp32-correctly-rounded-divide-sqrt"]
+# token.hip: no packed fp32 instructions (some of their forms have been seen to give wrong results on this GPU)
+SOURCE_FLAGS = {"token.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]}
 
 
 def _stale(lib, sources):
@@ -35,7 +37,7 @@ def _compile(jobs, verbose):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     procs = []
     for src, obj, extra in jobs:
-        cmd = [hipcc] + FLAGS + list(extra) + ["-c", os.path.join(CSRC, src), "-o", obj]
+        cmd = [hipcc] + FLAGS + SOURCE_FLAGS.get(src, []) + list(extra) + ["-c", os.path.join(CSRC, src), "-o", obj]
         if verbose:
             print(" ".join(cmd), flush=True)
         procs.append((subprocess.Popen(cmd), cmd))
