@@ -26,17 +26,73 @@
 #define RED_SEQ PPO_REDUCE_SEQUENCE_MEAN
 
 // ------------------------------------------------------------------------------------------ element types
-template <typename T> struct Vec {   // 16 bytes of a row
-    static constexpr int N = 16 / sizeof(T);
-    T v[N];
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// Element type and how 32 bits of a row hold it; 16 bytes are kept as four words, unpacked where they are used.
+template <typename T> struct Word;
+template <> struct Word<float> {
+    static constexpr int N = 1;
+    static __device__ __forceinline__ void unpack(uint32_t w, float* f) { f[0] = __uint_as_float(w); }
+    static __device__ __forceinline__ uint32_t pack(const float* f) { return __float_as_uint(f[0]); }
+    static constexpr uint32_t LOWEST = 0xff800000u;    // -inf
+};
+template <> struct Word<__bf16> {
+    static constexpr int N = 2;
+    static __device__ __forceinline__ void unpack(uint32_t w, float* f) {
+        f[0] = __uint_as_float(w << 16);
+        f[1] = __uint_as_float(w & 0xffff0000u);
+    }
+    static __device__ __forceinline__ uint32_t pack(const float* f) {   // to nearest even
+        const f32x2 v = {f[0], f[1]};
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+    }
+    static constexpr uint32_t LOWEST = 0xff80ff80u;
+};
+template <> struct Word<_Float16> {
+    static constexpr int N = 2;
+    static __device__ __forceinline__ void unpack(uint32_t w, float* f) {
+        const f16x2 h = __builtin_bit_cast(f16x2, w);
+        f[0] = (float)h.x;
+        f[1] = (float)h.y;
+    }
+    static __device__ __forceinline__ uint32_t pack(const float* f) {   // to nearest even
+        const f32x2 v = {f[0], f[1]};
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+    }
+    static constexpr uint32_t LOWEST = 0xfc00fc00u;
 };
 
-template <typename T> __device__ __forceinline__ Vec<T> load_vec(const T* p) {   // p: aligned for T only
-    Vec<T> o;
+template <typename T> constexpr int VEC = 4 * Word<T>::N;     // elements of 16 bytes
+
+template <typename T> __device__ __forceinline__ u32x4 load_vec(const T* p) {   // p: aligned for T only
+    u32x4 o;
     __builtin_memcpy(&o, p, 16);
     return o;
 }
-template <typename T> __device__ __forceinline__ void store_vec(T* p, const Vec<T>& o) { __builtin_memcpy(p, &o, 16); }
+template <typename T> __device__ __forceinline__ void store_vec(T* p, u32x4 o) { __builtin_memcpy(p, &o, 16); }
+
+// This thread's vector of the vectors that begin at a uniform address: one 32-bit offset for all
+// of a thread's accesses, the rest in scalar registers.
+template <typename T> __device__ __forceinline__ u32x4 load_at(const T* base) {
+    return load_vec((const T*)((const char*)base + threadIdx.x * 16u));
+}
+template <typename T> __device__ __forceinline__ void store_at(T* base, u32x4 o) {
+    store_vec((T*)((char*)base + threadIdx.x * 16u), o);
+}
+
+template <typename T> __device__ __forceinline__ void unpack(u32x4 v, float* f) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) Word<T>::unpack(v[k], f + k * Word<T>::N);
+}
+template <typename T> __device__ __forceinline__ u32x4 pack(const float* f) {
+    u32x4 v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = Word<T>::pack(f + k * Word<T>::N);
+    return v;
+}
 
 __device__ __forceinline__ float wide(float x) { return x; }
 __device__ __forceinline__ float wide(__bf16 x) { return (float)x; }
@@ -67,14 +123,6 @@ template <bool ENT> __device__ __forceinline__ void acc_rebase(Acc& a, float mn,
     a.m = mn;
 }
 
-template <bool ENT> __device__ __forceinline__ void acc_join(Acc& a, Acc b, float c2) {
-    const float mn = fmaxf(a.m, b.m);
-    acc_rebase<ENT>(a, mn, c2);
-    acc_rebase<ENT>(b, mn, c2);
-    a.s += b.s;
-    if (ENT) a.e += b.e;
-}
-
 template <bool ENT> __device__ __forceinline__ void acc_add(Acc& a, float x, float c2) {   // a.m >= x, or x is NaN
     const float u = (x - a.m) * c2;
     const float e = __builtin_amdgcn_exp2f(u);
@@ -82,49 +130,112 @@ template <bool ENT> __device__ __forceinline__ void acc_add(Acc& a, float x, flo
     if (ENT) a.e = fmaf(e, fmaxf(u, U_FLOOR), a.e);
 }
 
+// 16 * M bytes of logits at once: their maximum, one rescaling, their terms
+template <typename T, int M, bool ENT> __device__ __forceinline__ void acc_vecs(Acc& a, const u32x4* v, float c2) {
+    constexpr int N = VEC<T>;
+    float f[N * M], mx = a.m;
+#pragma unroll
+    for (int k = 0; k < M; ++k) unpack<T>(v[k], f + k * N);
+#pragma unroll
+    for (int i = 0; i < N * M; ++i) mx = fmaxf(mx, f[i]);
+    acc_rebase<ENT>(a, mx, c2);
+#pragma unroll
+    for (int i = 0; i < N * M; ++i) acc_add<ENT>(a, f[i], c2);
+}
+
+// Rotation within the 16 lanes of a row: an all-reduce in four steps without LDS.  Partners add the same two
+// numbers, so all lanes end with the same bits.
+template <int CTRL> __device__ __forceinline__ float ror(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float lane_value(float x, int lane) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
+}
+template <int W> __device__ __forceinline__ float row_max(float x) {   // of W = 1, 2, 4, 8, 16 lanes' values
+    if (W > 8) x = fmaxf(x, ror<0x128>(x));
+    if (W > 4) x = fmaxf(x, ror<0x124>(x));
+    if (W > 2) x = fmaxf(x, ror<0x122>(x));
+    if (W > 1) x = fmaxf(x, ror<0x121>(x));
+    return x;
+}
+template <int W> __device__ __forceinline__ float row_sum(float x) {
+    if (W > 8) x += ror<0x128>(x);
+    if (W > 4) x += ror<0x124>(x);
+    if (W > 2) x += ror<0x122>(x);
+    if (W > 1) x += ror<0x121>(x);
+    return x;
+}
+__device__ __forceinline__ float wave_max(float x) {
+    x = row_max<16>(x);
+    return fmaxf(fmaxf(lane_value(x, 0), lane_value(x, 16)), fmaxf(lane_value(x, 32), lane_value(x, 48)));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+    x = row_sum<16>(x);
+    return (lane_value(x, 0) + lane_value(x, 16)) + (lane_value(x, 32) + lane_value(x, 48));
+}
+
+// The threads' accumulators joined; every thread returns the same bits.  lds: NT / 64 entries.
 template <int NT, bool ENT> __device__ __forceinline__ Acc acc_block(Acc a, float c2, Acc* lds) {
     constexpr int W = NT / 64;
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-        Acc o;
-        o.m = __shfl_xor(a.m, off);
-        o.s = __shfl_xor(a.s, off);
-        o.e = ENT ? __shfl_xor(a.e, off) : 0.0f;
-        acc_join<ENT>(a, o, c2);
-    }
+    acc_rebase<ENT>(a, wave_max(a.m), c2);
+    a.s = wave_sum(a.s);
+    if (ENT) a.e = wave_sum(a.e);
     if (W == 1) return a;
     __syncthreads();          // the previous row's values have been read
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
     __syncthreads();
-    a = lds[0];
-#pragma unroll
-    for (int w = 1; w < W; ++w) acc_join<ENT>(a, lds[w], c2);
+    a = lds[threadIdx.x & (W - 1)];
+    acc_rebase<ENT>(a, row_max<W>(a.m), c2);
+    a.s = lane_value(row_sum<W>(a.s), 0);
+    if (ENT) a.e = lane_value(row_sum<W>(a.e), 0);
+    a.m = lane_value(a.m, 0);
     return a;
 }
 
-// (m, S, E) of a row by NT threads; every thread returns the same bits.
+// ------------------------------------------------------------------------------------------ a row on the chip
+// NT threads hold up to NT * HELD * 16 bytes of a row in registers, so that statistics and gradient read memory
+// once; the vectors beyond are read again for the gradient.  Vector j belongs to thread j % NT.  Vectors past the
+// end are filled with -inf, which adds nothing; the V % N last logits are one scalar of as many threads.
+#define HELD 16
+
+template <typename T, int NT> struct Row {
+    static constexpr int N = VEC<T>;
+    u32x4 v[HELD];
+    T tail;
+
+    __device__ __forceinline__ void load(const T* x, int V) {
+        const int nvec = V / N;
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            v[i] = Word<T>::LOWEST;
+            if ((int)threadIdx.x < nvec - i * NT) v[i] = load_at(x + i * NT * N);
+        }
+        tail = (T)-__builtin_inff();
+        if ((int)threadIdx.x < V - nvec * N) tail = x[nvec * N + threadIdx.x];
+    }
+};
+
+// vectors joined before each rescaling
+template <typename T> struct Step { static constexpr int M = sizeof(T) == 4 ? 4 : 2; };
+
 template <typename T, int NT, bool ENT>
-__device__ __forceinline__ Acc row_stats(const T* __restrict__ x, int V, float c2, Acc* lds) {
-    constexpr int N = Vec<T>::N;
+__device__ __forceinline__ Acc row_stats(const Row<T, NT>& row, const T* x, int V, float c2, Acc* lds) {
+    constexpr int N = VEC<T>, M = Step<T>::M;
     const int nvec = V / N;
     Acc a = acc_empty();
-    for (int j = threadIdx.x; j < nvec; j += NT) {
-        const Vec<T> v = load_vec(x + (int64_t)j * N);
-        float f[N], mx = a.m;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            f[i] = wide(v.v[i]);
-            mx = fmaxf(mx, f[i]);
+    for (int i = 0; i < HELD; i += M) {
+        if (i * NT >= nvec) break;
+        acc_vecs<T, M, ENT>(a, row.v + i, c2);
+    }
+    if (NT == 1024)
+        for (int j = HELD * NT + threadIdx.x; j < nvec; j += NT) {
+            const u32x4 v = load_vec(x + (int64_t)j * N);
+            acc_vecs<T, 1, ENT>(a, &v, c2);
         }
-        acc_rebase<ENT>(a, mx, c2);
-#pragma unroll
-        for (int i = 0; i < N; ++i) acc_add<ENT>(a, f[i], c2);
-    }
-    for (int i = nvec * N + threadIdx.x; i < V; i += NT) {
-        const float f = wide(x[i]);
-        acc_rebase<ENT>(a, fmaxf(a.m, f), c2);
-        acc_add<ENT>(a, f, c2);
-    }
+    const float t = wide(row.tail);
+    acc_rebase<ENT>(a, fmaxf(a.m, t), c2);
+    acc_add<ENT>(a, t, c2);
     return acc_block<NT, ENT>(a, c2, lds);
 }
 
@@ -141,34 +252,60 @@ template <bool ENT> __device__ __forceinline__ float grad_of(const RowGrad& g, f
     return ENT ? e * fmaf(g.b, fmaxf(u, U_FLOOR), g.a) : e * g.a;
 }
 
-template <typename T, int NT, bool ENT>
-__device__ __forceinline__ void row_grad(const T* x, T* out, int V, float c2, const RowGrad& g) {   // x may be out
-    constexpr int N = Vec<T>::N;
-    const int nvec = V / N;
-    for (int j = threadIdx.x; j < nvec; j += NT) {
-        const Vec<T> v = load_vec(x + (int64_t)j * N);
-        Vec<T> o;
+template <typename T, bool ENT>
+__device__ __forceinline__ u32x4 grad_vec(const RowGrad& g, u32x4 v, int j, float c2) {
+    constexpr int N = VEC<T>;
+    float d[N];
+    unpack<T>(v, d);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float d = grad_of<ENT>(g, wide(v.v[i]), c2);
-            if (j * N + i == g.tok) d += g.gt;
-            o.v[i] = (T)d;    // the one rounding of the gradient, to nearest even
-        }
-        store_vec(out + (int64_t)j * N, o);
+    for (int i = 0; i < N; ++i) d[i] = grad_of<ENT>(g, d[i], c2);
+    if (j == g.tok / N && g.tok >= 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) d[i] += i == g.tok % N ? g.gt : 0.0f;
     }
-    for (int i = nvec * N + threadIdx.x; i < V; i += NT) {
-        float d = grad_of<ENT>(g, wide(x[i]), c2);
-        if (i == g.tok) d += g.gt;
-        out[i] = (T)d;
+    return pack<T>(d);        // the one rounding of the gradient
+}
+
+template <typename T, bool ENT> __device__ __forceinline__ T grad_one(const RowGrad& g, T x, int i, float c2) {
+    const float d = grad_of<ENT>(g, wide(x), c2);
+    return (T)(i == g.tok ? d + g.gt : d);
+}
+
+// the gradient of a held row; the vectors that are read again may lie where the gradient goes
+template <typename T, int NT, bool ENT>
+__device__ __forceinline__ void row_grad(const Row<T, NT>& row, const T* x, T* out, int V, float c2, const RowGrad& g) {
+    constexpr int N = VEC<T>;
+    const int nvec = V / N;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        if (i * NT >= nvec) break;
+        const u32x4 o = grad_vec<T, ENT>(g, row.v[i], i * NT + threadIdx.x, c2);
+        if ((int)threadIdx.x < nvec - i * NT) store_at(out + i * NT * N, o);
     }
+    if (NT == 1024)
+        for (int j = HELD * NT + threadIdx.x; j < nvec; j += NT)
+            store_vec(out + (int64_t)j * N, grad_vec<T, ENT>(g, load_vec(x + (int64_t)j * N), j, c2));
+    const int i = nvec * N + threadIdx.x;
+    if (i < V) out[i] = grad_one<T, ENT>(g, row.tail, i, c2);
+}
+
+// the gradient of a row whose statistics are known; x may be out
+template <typename T, int NT, bool ENT>
+__device__ __forceinline__ void row_map(const T* x, T* out, int V, float c2, const RowGrad& g) {
+    constexpr int N = VEC<T>;
+    const int nvec = V / N;
+    for (int j = threadIdx.x; j < nvec; j += NT)
+        store_vec(out + (int64_t)j * N, grad_vec<T, ENT>(g, load_vec(x + (int64_t)j * N), j, c2));
+    for (int i = nvec * N + threadIdx.x; i < V; i += NT) out[i] = grad_one<T, ENT>(g, x[i], i, c2);
 }
 
 template <typename T, int NT> __device__ __forceinline__ void row_fill(T* out, int V, float value) {
-    constexpr int N = Vec<T>::N;
+    constexpr int N = VEC<T>;
     const int nvec = V / N;
-    Vec<T> o;
+    float f[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) o.v[i] = (T)value;
+    for (int i = 0; i < N; ++i) f[i] = value;
+    const u32x4 o = pack<T>(f);
     for (int j = threadIdx.x; j < nvec; j += NT) store_vec(out + (int64_t)j * N, o);
     for (int i = nvec * N + threadIdx.x; i < V; i += NT) out[i] = (T)value;
 }
@@ -211,12 +348,19 @@ struct RowStats {             // what the backward pass needs of the forward pas
     float m, s, h, w;
 };
 
-// ln S with an absolute error of 2^-24: the exponent is taken apart, log2 acts on [1, 2)
+// ln S in fp64: S = 2^k f, f in [1/sqrt 2, sqrt 2), ln f = 2 artanh((f - 1) / (f + 1)) by its series (|argument| < 0.172:
+// the first term left out is below 2e-11)
 __device__ __forceinline__ double ln_of(float s) {
     int k;
-    const float f = frexpf(s, &k);
+    float f = frexpf(s, &k);
     if (!(s > 0.0f) || isinf(s)) return (double)logf(s);
-    return ((double)(k - 1) + (double)log2f(2.0f * f)) * LN2_D;
+    if (f < 0.70710678f) {
+        f *= 2.0f;
+        k -= 1;
+    }
+    const double z = ((double)f - 1.0) / ((double)f + 1.0), y = z * z;
+    const double p = fma(y, fma(y, fma(y, fma(y, fma(y, 1.0 / 11, 1.0 / 9), 1.0 / 7), 1.0 / 5), 1.0 / 3), 1.0);
+    return fma((double)k, LN2_D, 2.0 * z * p);
 }
 
 // log-probability of `tok`, NaN for one that is not in the vocabulary (its row of logits is not indexed with it)
@@ -284,7 +428,7 @@ __global__ __launch_bounds__(1024) void total_kernel(const double* __restrict__ 
 
 // ------------------------------------------------------------------------------------------ log-probabilities
 template <typename T, int NT, bool ENT>
-__global__ __launch_bounds__(NT) void logprobs_kernel(Logits L, const void* tokens, int i64, const uint8_t* mask,
+__global__ __launch_bounds__(NT, 4) void logprobs_kernel(Logits L, const void* tokens, int i64, const uint8_t* mask,
                                                       float* logprobs, double* logprobs64, float* entropy,
                                                       RowStats* stats) {
     __shared__ Acc lds[NT / 64];
@@ -294,7 +438,9 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Logits L, const void* toke
         RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
         if (!mask || mask[r]) {
             const T* x = row_in<T>(L, b, t);
-            const Acc a = row_stats<T, NT, ENT>(x, L.V, L.c2, lds);
+            Row<T, NT> row;
+            row.load(x, L.V);
+            const Acc a = row_stats<T, NT, ENT>(row, x, L.V, L.c2, lds);
             const double ln_s = ln_of(a.s);
             lp = token_logp(x, int_at(tokens, i64, r), L.V, L.c, a, ln_s);
             st.m = a.m;
@@ -329,7 +475,7 @@ struct Incoming {             // dL/dlogp and dL/dH of each row, and a factor on
 };
 
 template <typename T, int NT, bool ENT>
-__global__ __launch_bounds__(NT) void backward_kernel(Logits L, const void* tokens, int i64, const uint8_t* mask,
+__global__ __launch_bounds__(NT, 4) void backward_kernel(Logits L, const void* tokens, int i64, const uint8_t* mask,
                                                       const RowStats* __restrict__ stats, Incoming in) {
     const float f = in.factor ? *in.factor : 1.0f;
     for (int64_t r = blockIdx.x; r < L.n; r += gridDim.x) {
@@ -343,7 +489,7 @@ __global__ __launch_bounds__(NT) void backward_kernel(Logits L, const void* toke
         const float g_lp = in.lp ? f * in.lp[b * in.lp_s + t * in.lp_t] : 0.0f;
         const float g_h = ENT ? f * in.h[b * in.h_s + t * in.h_t] : 0.0f;
         const RowGrad g = grad_seed(st.m, st.s, st.h, g_lp, g_h, int_at(tokens, i64, r), L.V, L.c);
-        row_grad<T, NT, ENT>(row_in<T>(L, b, t), out, L.V, L.c2, g);
+        row_map<T, NT, ENT>(row_in<T>(L, b, t), out, L.V, L.c2, g);
     }
 }
 
@@ -362,18 +508,19 @@ struct PolicyArgs {
 };
 
 struct PolicyRow {
-    float loss, g_lp, g_h;    // weighted
+    double loss;              // weighted, as the gradients are
+    float g_lp, g_h;
 };
 
 __device__ __forceinline__ PolicyRow policy_row(const PolicyArgs& p, double lp, float h, float old_lp, float adv,
                                                 float ref, float w) {
-    // differences of log-probabilities are formed in fp64, where they lose nothing; the rest is fp32
-    const float r = expf((float)(lp - (double)old_lp));
-    const float s1 = r * adv, s2 = fminf(fmaxf(r, p.lo), p.hi) * adv;
-    const bool clipped = (adv > 0.0f && r > p.hi) || (adv < 0.0f && r < p.lo);
-    PolicyRow o;
-    o.loss = -(clipped ? s2 : s1);
-    float g = clipped ? 0.0f : -s1;
+    // Differences of log-probabilities are formed in fp64, where they lose nothing.  The ratio is 1 + (e^d - 1) with
+    // the second part in fp32: near 1 that keeps more of it than fp32 does, and a loss is a mean in which A and -A
+    // nearly cancel.
+    const double r = 1.0 + (double)expm1f((float)(lp - (double)old_lp)), a = (double)adv;
+    const bool clipped = (adv > 0.0f && r > (double)p.hi) || (adv < 0.0f && r < (double)p.lo);
+    double loss = clipped ? -(adv > 0.0f ? (double)p.hi : (double)p.lo) * a : -r * a;
+    float g = clipped ? 0.0f : (float)(-r * a);
     if (p.kl != 0.0f) {
         const float d = (float)((double)ref - lp);
         // e^d - 1 - d: its series where the difference would cancel (|d|^6 / 20160 < 2^-24 at 1/4)
@@ -381,28 +528,27 @@ __device__ __forceinline__ PolicyRow policy_row(const PolicyArgs& p, double lp, 
         const float k = fabsf(d) < 0.25f
             ? d * d * fmaf(d, fmaf(d, fmaf(d, fmaf(d, fmaf(d, 1.0f / 5040, 1.0f / 720), 1.0f / 120), 1.0f / 24), 1.0f / 6), 0.5f)
             : em1 - d;
-        o.loss = fmaf(p.kl, k, o.loss);
+        loss = fma((double)p.kl, (double)k, loss);
         g = fmaf(-p.kl, em1, g);
     }
-    if (p.ent != 0.0f) o.loss = fmaf(-p.ent, h, o.loss);
-    o.loss *= w;
-    o.g_lp = w * g;
-    o.g_h = -w * p.ent;
-    return o;
+    if (p.ent != 0.0f) loss = fma(-(double)p.ent, (double)h, loss);
+    return {loss * (double)w, w * g, -w * p.ent};
 }
 
 template <typename T, int NT, bool GRAD, bool ENT_GRAD>
-__global__ __launch_bounds__(NT) void policy_kernel(Logits L, PolicyArgs p) {
+__global__ __launch_bounds__(NT, 4) void policy_kernel(Logits L, PolicyArgs p) {
     __shared__ Acc lds[NT / 64];
     double total = 0.0;
     for (int64_t r = blockIdx.x; r < L.n; r += gridDim.x) {
         const int64_t b = r / L.n_tok, t = r - b * L.n_tok;
         RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
         double lp = 0.0;
-        PolicyRow o = {0.0f, 0.0f, 0.0f};
+        PolicyRow o = {0.0, 0.0f, 0.0f};
         if (!p.w.mask || p.w.mask[r]) {
             const T* x = row_in<T>(L, b, t);
-            const Acc a = row_stats<T, NT, true>(x, L.V, L.c2, lds);
+            Row<T, NT> row;
+            row.load(x, L.V);
+            const Acc a = row_stats<T, NT, true>(row, x, L.V, L.c2, lds);
             const double ln_s = ln_of(a.s);
             const int64_t tok = int_at(p.tokens, p.i64, r);
             lp = token_logp(x, tok, L.V, L.c, a, ln_s);
@@ -411,10 +557,10 @@ __global__ __launch_bounds__(NT) void policy_kernel(Logits L, PolicyArgs p) {
             st.h = (float)(ln_s - LN2_D * (double)(a.e / a.s));
             o = policy_row(p, lp, st.h, p.old_lp[r], p.adv[b * p.adv_s + t * p.adv_t], p.ref ? p.ref[r] : 0.0f,
                            row_weight(p.w, b, L.n_tok));
-            total += (double)o.loss;
+            total += o.loss;
             if (GRAD) {
                 __syncthreads();   // x[tok] has been read by all: the gradient may overwrite the logits
-                row_grad<T, NT, ENT_GRAD>(x, row_out<T>(L, b, t), L.V, L.c2,
+                row_grad<T, NT, ENT_GRAD>(row, x, row_out<T>(L, b, t), L.V, L.c2,
                                           grad_seed(a.m, a.s, st.h, o.g_lp, o.g_h, tok, L.V, L.c));
             }
         } else if (GRAD) {
@@ -484,20 +630,21 @@ struct Teacher {              // one row's entries, in LDS
     float q[PPO_MAX_TEACHER_TOP];       // teacher's probability of the entry
     float all[PPO_MAX_TEACHER_TOP];     // the same summed over the entries of this index
     float u[PPO_MAX_TEACHER_TOP];       // the student's logit there
-    float red[32];
-    int bad;
+    float entropy, loss;                // sum q ln q; the row's loss
+    int bad, some;                      // a token beyond the vocabulary; an entry that is not padding
 };
 
 // Reads the row's entries and makes them probabilities; two barriers at least lie before any of it is used.
 template <typename T, int NT>
 __device__ __forceinline__ void teacher_load(const TeacherArgs& p, const Logits& L, int64_t r, const T* x, Teacher& s) {
     __syncthreads();          // the previous row's entries have been used
-    if (threadIdx.x == 0) s.bad = 0;
+    if (threadIdx.x == 0) s.bad = s.some = 0;
     __syncthreads();
     for (int k = threadIdx.x; k < p.K; k += NT) {
         const int64_t i = int_at(p.index, p.i64, r * p.K + k);
         const bool there = i >= 0 && i < L.V;
         if (i >= L.V) s.bad = 1;
+        if (there) s.some = 1;
         s.index[k] = there ? (int)i : -1;
         s.q[k] = there ? float_at(p.logit, p.dtype, r * p.K + k) : 0.0f;
         s.u[k] = there ? wide(x[i]) : 0.0f;
@@ -527,7 +674,7 @@ __device__ __forceinline__ void teacher_load(const TeacherArgs& p, const Logits&
         }
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) ent += __shfl_xor(ent, off);
-        if (threadIdx.x == 0) s.red[0] = ent;
+        if (threadIdx.x == 0) s.entropy = ent;
     }
     __syncthreads();
     for (int k = threadIdx.x; k < p.K; k += NT) {
@@ -547,24 +694,21 @@ __device__ __forceinline__ float teacher_loss(const TeacherArgs& p, Teacher& s, 
                 cross += (double)s.q[k] * (((double)s.u[k] - (double)m) * (double)c - ln_s);
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) cross += __shfl_xor(cross, off);
-        if (threadIdx.x == 0) s.red[1] = s.bad ? __builtin_nanf("") : (float)((double)s.red[0] - cross);
+        if (threadIdx.x == 0) s.loss = s.bad ? __builtin_nanf("") : (float)((double)s.entropy - cross);
     }
     __syncthreads();
-    return s.red[1];
+    return s.loss;
 }
 
-// dL/dx_i = g (p_i - sum of the teacher's q at i): the bulk first, the K places after a barrier
+// dL/dx_i = g (p_i - sum of the teacher's q at i): the bulk first, the K places after a barrier.  A teacher that gave
+// nothing teaches nothing.
+__device__ __forceinline__ RowGrad teacher_seed(const Teacher& s, float m, float sum, float g) {
+    return {m, s.bad ? __builtin_nanf("") : s.some ? g / sum : 0.0f, 0.0f, 0.0f, -1};
+}
+
 template <typename T, int NT>
-__device__ __forceinline__ void teacher_grad(const TeacherArgs& p, const Teacher& s, const T* x, T* out,
-                                             const Logits& L, float m, float sum, float g) {
-    bool any = false;
-    for (int k = 0; k < p.K; ++k) any |= s.index[k] >= 0;
-    if (!any && !s.bad) {     // a teacher that gave nothing teaches nothing
-        row_fill<T, NT>(out, L.V, 0.0f);
-        return;
-    }
-    const RowGrad rg = {m, s.bad ? __builtin_nanf("") : g / sum, 0.0f, 0.0f, -1};
-    row_grad<T, NT, false>(x, out, L.V, L.c2, rg);
+__device__ __forceinline__ void teacher_places(const TeacherArgs& p, const Teacher& s, T* out, const Logits& L,
+                                               const RowGrad& rg, float g) {
     __syncthreads();          // the bulk is written
     if (s.bad) return;
     for (int k = threadIdx.x; k < p.K; k += NT)
@@ -572,7 +716,7 @@ __device__ __forceinline__ void teacher_grad(const TeacherArgs& p, const Teacher
 }
 
 template <typename T, int NT, bool GRAD>
-__global__ __launch_bounds__(NT) void distill_kernel(Logits L, TeacherArgs p) {
+__global__ __launch_bounds__(NT, 4) void distill_kernel(Logits L, TeacherArgs p) {
     __shared__ Acc lds[NT / 64];
     __shared__ Teacher teach;
     const float temp = 1.0f / L.c;
@@ -583,14 +727,21 @@ __global__ __launch_bounds__(NT) void distill_kernel(Logits L, TeacherArgs p) {
         float loss = 0.0f;
         if (!p.w.mask || p.w.mask[r]) {
             const T* x = row_in<T>(L, b, t);
+            Row<T, NT> row;
+            row.load(x, L.V);
             teacher_load<T, NT>(p, L, r, x, teach);
-            const Acc a = row_stats<T, NT, false>(x, L.V, L.c2, lds);
+            const Acc a = row_stats<T, NT, false>(row, x, L.V, L.c2, lds);
             loss = temp * temp * teacher_loss(p, teach, a.m, L.c, ln_of(a.s));
             st.m = a.m;
             st.s = a.s;
             st.w = row_weight(p.w, b, L.n_tok);
             total += (double)st.w * (double)loss;
-            if (GRAD) teacher_grad<T, NT>(p, teach, x, row_out<T>(L, b, t), L, a.m, a.s, st.w * temp);
+            if (GRAD) {
+                T* out = row_out<T>(L, b, t);
+                const RowGrad g = teacher_seed(teach, a.m, a.s, st.w * temp);
+                row_grad<T, NT, false>(row, x, out, L.V, L.c2, g);
+                teacher_places<T, NT>(p, teach, out, L, g, st.w * temp);
+            }
         } else if (GRAD) {
             row_fill<T, NT>(row_out<T>(L, b, t), L.V, 0.0f);
         }
@@ -603,7 +754,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(Logits L, TeacherArgs p) {
 }
 
 template <typename T, int NT>
-__global__ __launch_bounds__(NT) void distill_backward_kernel(Logits L, TeacherArgs p) {
+__global__ __launch_bounds__(NT, 4) void distill_backward_kernel(Logits L, TeacherArgs p) {
     __shared__ Teacher teach;
     const float f = (p.factor ? *p.factor : 1.0f) / L.c;
     for (int64_t r = blockIdx.x; r < L.n; r += gridDim.x) {
@@ -617,7 +768,9 @@ __global__ __launch_bounds__(NT) void distill_backward_kernel(Logits L, TeacherA
         const RowStats st = p.stats[r];
         teacher_load<T, NT>(p, L, r, x, teach);
         __syncthreads();
-        teacher_grad<T, NT>(p, teach, x, out, L, st.m, st.s, f * st.w);
+        const RowGrad g = teacher_seed(teach, st.m, st.s, f * st.w);
+        row_map<T, NT, false>(x, out, L.V, L.c2, g);
+        teacher_places<T, NT>(p, teach, out, L, g, f * st.w);
     }
 }
 
@@ -687,11 +840,29 @@ static Logits logits_of(const ppo_token_logits* x, void* grad) {
 
 static int grid_of(int64_t n) { return (int)(n < MAX_GRID ? n : MAX_GRID); }
 
-#define NT 256
 #define BY_TYPE(dtype, T, ...)                                                     \
     if ((dtype) == PPO_F32) { using T = float; __VA_ARGS__; }                      \
     else if ((dtype) == PPO_BF16) { using T = __bf16; __VA_ARGS__; }               \
     else { using T = _Float16; __VA_ARGS__; }
+
+// Threads of a row: as few as hold it (a row is then in flight as a whole, and the more rows a CU has under way, the
+// more of one's memory time hides another's arithmetic).
+static int threads_of(const Logits& L, int dtype) {
+    const int64_t bytes = (int64_t)L.V * (dtype == PPO_F32 ? 4 : 2);
+    int nt = 64;
+    while (nt < 1024 && (int64_t)nt * HELD * 16 < bytes) nt *= 2;
+    return nt;
+}
+
+#define BY_THREADS(threads, NT, ...)                                               \
+    switch (threads) {                                                             \
+        case 64: { constexpr int NT = 64; __VA_ARGS__; break; }                    \
+        case 128: { constexpr int NT = 128; __VA_ARGS__; break; }                  \
+        case 256: { constexpr int NT = 256; __VA_ARGS__; break; }                  \
+        case 512: { constexpr int NT = 512; __VA_ARGS__; break; }                  \
+        default: { constexpr int NT = 1024; __VA_ARGS__; break; }                  \
+    }
+#define BY_TYPE_AND_THREADS(dtype, threads, T, NT, ...) BY_TYPE(dtype, T, BY_THREADS(threads, NT, __VA_ARGS__))
 
 // Counted rows of each sequence and of all, where a weight needs them.
 static void count_rows(const uint8_t* mask, int reduction, const ppo_token_logits* x, const Workspace& w, hipStream_t st) {
@@ -719,7 +890,7 @@ extern "C" int ppo_token_logprobs(const ppo_token_logits* x, const void* tokens,
     const Logits L = logits_of(x, nullptr);
     if (L.n == 0) return 0;
     if (!tokens || !logprobs) return PPO_E_BADARG;
-    BY_TYPE(x->dtype, T, {
+    BY_TYPE_AND_THREADS(x->dtype, threads_of(L, x->dtype), T, NT, {
         if (entropy) logprobs_kernel<T, NT, true><<<grid_of(L.n), NT, 0, (hipStream_t)stream>>>(
             L, tokens, tokens_are_i64, mask, logprobs, nullptr, entropy, (RowStats*)row_stats);
         else logprobs_kernel<T, NT, false><<<grid_of(L.n), NT, 0, (hipStream_t)stream>>>(
@@ -730,6 +901,7 @@ extern "C" int ppo_token_logprobs(const ppo_token_logits* x, const void* tokens,
 
 static int launch_backward(const Logits& L, int dtype, const void* tokens, int i64, const uint8_t* mask,
                            const RowStats* stats, const Incoming& in, hipStream_t st) {
+    constexpr int NT = 256;
     BY_TYPE(dtype, T, {
         if (in.h) backward_kernel<T, NT, true><<<grid_of(L.n), NT, 0, st>>>(L, tokens, i64, mask, stats, in);
         else backward_kernel<T, NT, false><<<grid_of(L.n), NT, 0, st>>>(L, tokens, i64, mask, stats, in);
@@ -787,7 +959,7 @@ extern "C" int ppo_policy_loss(const ppo_token_logits* x, const void* tokens, in
         p.g_h = seeds ? seeds + L.n : nullptr;
         p.part = w.part;
         count_rows(mask, terms->reduction, x, w, st);
-        BY_TYPE(x->dtype, T, {
+        BY_TYPE_AND_THREADS(x->dtype, threads_of(L, x->dtype), T, NT, {
             if (!grad) policy_kernel<T, NT, false, false><<<grid_of(L.n), NT, 0, st>>>(L, p);
             else if (p.ent != 0.0f) policy_kernel<T, NT, true, true><<<grid_of(L.n), NT, 0, st>>>(L, p);
             else policy_kernel<T, NT, true, false><<<grid_of(L.n), NT, 0, st>>>(L, p);
@@ -813,7 +985,7 @@ extern "C" int ppo_preference_loss(const ppo_token_logits* x, const void* tokens
     RowStats* stats = row_stats ? (RowStats*)row_stats : w.stats;
     float* sd = seeds ? seeds : w.seeds;
     if (L.n > 0) {
-        BY_TYPE(x->dtype, T, (logprobs_kernel<T, NT, false><<<grid_of(L.n), NT, 0, st>>>(
+        BY_TYPE_AND_THREADS(x->dtype, threads_of(L, x->dtype), T, NT, (logprobs_kernel<T, NT, false><<<grid_of(L.n), NT, 0, st>>>(
             L, tokens, tokens_are_i64, mask, nullptr, w.lp64, nullptr, stats)))
     }
     pair_kernel<<<grid_of(pairs), 256, 0, st>>>(w.lp64, mask, ref_logprobs, pairs, x->n_tok, beta, label_smoothing, scale,
@@ -861,7 +1033,7 @@ extern "C" int ppo_distillation_loss(const ppo_token_logits* x, const void* teac
     p.part = w.part;
     if (L.n > 0) {
         count_rows(mask, reduction, x, w, st);
-        BY_TYPE(x->dtype, T, {
+        BY_TYPE_AND_THREADS(x->dtype, threads_of(L, x->dtype), T, NT, {
             if (grad) distill_kernel<T, NT, true><<<grid_of(L.n), NT, 0, st>>>(L, p);
             else distill_kernel<T, NT, false><<<grid_of(L.n), NT, 0, st>>>(L, p);
         })
@@ -883,6 +1055,7 @@ extern "C" int ppo_distillation_backward(const ppo_token_logits* x, const void* 
     p.w.mask = mask;
     p.stats = (RowStats*)row_stats;
     p.factor = grad_factor;
+    constexpr int NT = 256;
     BY_TYPE(x->dtype, T, (distill_backward_kernel<T, NT><<<grid_of(L.n), NT, 0, (hipStream_t)stream>>>(L, p)))
     return (int)hipGetLastError();
 }
