@@ -335,7 +335,7 @@ int ppo_update_epochs(float* params, int state_dim, int action_dim, int continuo
 #define PPO_F32 0
 #define PPO_BF16 1
 #define PPO_F16 2
-#define PPO_MAX_VOCAB (1 << 30)
+#define PPO_MAX_VOCAB (1 << 26)
 #define PPO_MAX_TOKENS (1 << 30)       /* rows of one call */
 #define PPO_MAX_TEACHER_TOP 512
 

@@ -19,7 +19,6 @@
 #define LOG2E_F 1.4426950408889634f
 #define LN2_D 0.6931471805599453
 #define U_FLOOR (-1.0e6f)    // below it e_i is 0: products e_i u_i take this in place of -inf
-#define MAX_GRID 8192        // workgroups of a launch; rows beyond are taken in turns
 
 #define RED_SUM PPO_REDUCE_SUM
 #define RED_TOKEN PPO_REDUCE_TOKEN_MEAN
@@ -67,22 +66,6 @@ template <> struct Word<_Float16> {
 
 template <typename T> constexpr int VEC = 4 * Word<T>::N;     // elements of 16 bytes
 
-template <typename T> __device__ __forceinline__ u32x4 load_vec(const T* p) {   // p: aligned for T only
-    u32x4 o;
-    __builtin_memcpy(&o, p, 16);
-    return o;
-}
-template <typename T> __device__ __forceinline__ void store_vec(T* p, u32x4 o) { __builtin_memcpy(p, &o, 16); }
-
-// This thread's vector of the vectors that begin at a uniform address: one 32-bit offset for all
-// of a thread's accesses, the rest in scalar registers.
-template <typename T> __device__ __forceinline__ u32x4 load_at(const T* base) {
-    return load_vec((const T*)((const char*)base + threadIdx.x * 16u));
-}
-template <typename T> __device__ __forceinline__ void store_at(T* base, u32x4 o) {
-    store_vec((T*)((char*)base + threadIdx.x * 16u), o);
-}
-
 template <typename T> __device__ __forceinline__ void unpack(u32x4 v, float* f) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) Word<T>::unpack(v[k], f + k * Word<T>::N);
@@ -110,37 +93,53 @@ __device__ __forceinline__ float float_at(const void* p, int dtype, int64_t i) {
 // ------------------------------------------------------------------------------------------ row statistics
 struct Acc {
     float m, s, e;
+    float n;                  // counted rows of the mask, where a kernel counts them itself
 };
 
-__device__ __forceinline__ Acc acc_empty() { return {-__FLT_MAX__, 0.0f, 0.0f}; }   // finite: -inf logits give u = -inf
+__device__ __forceinline__ Acc acc_empty() { return {-__FLT_MAX__, 0.0f, 0.0f, 0.0f}; }   // finite: -inf logits give u = -inf
+
+// u_i has two forms.  Exact: (x - m) c2.  NEAR: fma(x, c2, -M) with M = m c2 rounded, one instruction less for each
+// logit; what M is off by, at most 2^-24 |M|, is the same for all terms of a row and is put back by near_done().  It
+// needs |M| < NEAR_LIMIT: rows beyond (logits of a million and more, rows of nothing but -inf) are done over exactly.
+#define NEAR_LIMIT 1048576.0f
+__device__ __forceinline__ float near_max(float m, float c2) { return fmaxf(m * c2, -NEAR_LIMIT); }
+__device__ __forceinline__ bool is_near(float m, float c2) { return fabsf(m * c2) < NEAR_LIMIT; }
 
 // a, relative to a larger maximum mn
-template <bool ENT> __device__ __forceinline__ void acc_rebase(Acc& a, float mn, float c2) {
-    const float d = fmaxf((a.m - mn) * c2, -1.0e30f);
+template <bool ENT, bool NEAR = false> __device__ __forceinline__ void acc_rebase(Acc& a, float mn, float c2) {
+    const float d = NEAR ? near_max(a.m, c2) - near_max(mn, c2) : fmaxf((a.m - mn) * c2, -1.0e30f);
     const float r = __builtin_amdgcn_exp2f(d);
-    if (ENT) a.e = (a.e + a.s * d) * r;
+    if (ENT) a.e = fmaf(a.s, d, a.e) * r;
     a.s *= r;
     a.m = mn;
 }
 
-template <bool ENT> __device__ __forceinline__ void acc_add(Acc& a, float x, float c2) {   // a.m >= x, or x is NaN
-    const float u = (x - a.m) * c2;
+template <bool ENT, bool NEAR = false> __device__ __forceinline__ void acc_add(Acc& a, float x, float c2) {   // a.m >= x, or x is NaN
+    const float u = NEAR ? fmaf(x, c2, -near_max(a.m, c2)) : (x - a.m) * c2;
     const float e = __builtin_amdgcn_exp2f(u);
     a.s += e;
     if (ENT) a.e = fmaf(e, fmaxf(u, U_FLOOR), a.e);
 }
 
 // 16 * M bytes of logits at once: their maximum, one rescaling, their terms
-template <typename T, int M, bool ENT> __device__ __forceinline__ void acc_vecs(Acc& a, const u32x4* v, float c2) {
+template <typename T, int M, bool ENT, bool NEAR = false>
+__device__ __forceinline__ void acc_vecs(Acc& a, const u32x4* v, float c2) {
     constexpr int N = VEC<T>;
     float f[N * M], mx = a.m;
 #pragma unroll
     for (int k = 0; k < M; ++k) unpack<T>(v[k], f + k * N);
 #pragma unroll
     for (int i = 0; i < N * M; ++i) mx = fmaxf(mx, f[i]);
-    acc_rebase<ENT>(a, mx, c2);
+    acc_rebase<ENT, NEAR>(a, mx, c2);
 #pragma unroll
-    for (int i = 0; i < N * M; ++i) acc_add<ENT>(a, f[i], c2);
+    for (int i = 0; i < N * M; ++i) acc_add<ENT, NEAR>(a, f[i], c2);
+}
+
+// The sums as they are relative to m c2 itself: with rho = m c2 - M the terms are e_i 2^-rho, u_i - rho.
+__device__ __forceinline__ Acc near_done(Acc a, float c2) {
+    const float rho = (float)((double)a.m * (double)c2 - (double)near_max(a.m, c2));
+    const float f = __builtin_amdgcn_exp2f(-rho);
+    return {a.m, a.s * f, (a.e - rho * a.s) * f, a.n};
 }
 
 // Rotation within the 16 lanes of a row: an all-reduce in four steps without LDS.  Partners add the same two
@@ -151,92 +150,196 @@ template <int CTRL> __device__ __forceinline__ float ror(float x) {
 __device__ __forceinline__ float lane_value(float x, int lane) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
 }
-template <int W> __device__ __forceinline__ float row_max(float x) {   // of W = 1, 2, 4, 8, 16 lanes' values
-    if (W > 8) x = fmaxf(x, ror<0x128>(x));
-    if (W > 4) x = fmaxf(x, ror<0x124>(x));
-    if (W > 2) x = fmaxf(x, ror<0x122>(x));
-    if (W > 1) x = fmaxf(x, ror<0x121>(x));
-    return x;
+__device__ __forceinline__ float row_max(float x) {
+    x = fmaxf(x, ror<0x128>(x));
+    x = fmaxf(x, ror<0x124>(x));
+    x = fmaxf(x, ror<0x122>(x));
+    return fmaxf(x, ror<0x121>(x));
 }
-template <int W> __device__ __forceinline__ float row_sum(float x) {
-    if (W > 8) x += ror<0x128>(x);
-    if (W > 4) x += ror<0x124>(x);
-    if (W > 2) x += ror<0x122>(x);
-    if (W > 1) x += ror<0x121>(x);
-    return x;
+__device__ __forceinline__ float row_sum(float x) {
+    x += ror<0x128>(x);
+    x += ror<0x124>(x);
+    x += ror<0x122>(x);
+    return x + ror<0x121>(x);
 }
 __device__ __forceinline__ float wave_max(float x) {
-    x = row_max<16>(x);
+    x = row_max(x);
     return fmaxf(fmaxf(lane_value(x, 0), lane_value(x, 16)), fmaxf(lane_value(x, 32), lane_value(x, 48)));
 }
 __device__ __forceinline__ float wave_sum(float x) {
-    x = row_sum<16>(x);
+    x = row_sum(x);
     return (lane_value(x, 0) + lane_value(x, 16)) + (lane_value(x, 32) + lane_value(x, 48));
 }
 
-// The threads' accumulators joined; every thread returns the same bits.  lds: NT / 64 entries.
-template <int NT, bool ENT> __device__ __forceinline__ Acc acc_block(Acc a, float c2, Acc* lds) {
-    constexpr int W = NT / 64;
-    acc_rebase<ENT>(a, wave_max(a.m), c2);
+// The accumulators of a wave's lanes joined, the same bits in every lane.
+template <bool ENT, bool NEAR = false> __device__ __forceinline__ Acc acc_wave(Acc a, float c2) {
+    acc_rebase<ENT, NEAR>(a, wave_max(a.m), c2);
     a.s = wave_sum(a.s);
     if (ENT) a.e = wave_sum(a.e);
-    if (W == 1) return a;
-    __syncthreads();          // the previous row's values have been read
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
-    __syncthreads();
-    a = lds[threadIdx.x & (W - 1)];
-    acc_rebase<ENT>(a, row_max<W>(a.m), c2);
-    a.s = lane_value(row_sum<W>(a.s), 0);
-    if (ENT) a.e = lane_value(row_sum<W>(a.e), 0);
-    a.m = lane_value(a.m, 0);
+    a.n = wave_sum(a.n);
     return a;
 }
 
-// ------------------------------------------------------------------------------------------ a row on the chip
-// NT threads hold up to NT * HELD * 16 bytes of a row in registers, so that statistics and gradient read memory
-// once; the vectors beyond are read again for the gradient.  Vector j belongs to thread j % NT.  Vectors past the
-// end are filled with -inf, which adds nothing; the V % N last logits are one scalar of as many threads.
-#define HELD 16
+// And those of the workgroup's waves (at most 16), which lie in lds.
+template <bool ENT, bool NEAR = false> __device__ __forceinline__ Acc acc_waves(const Acc* lds, float c2) {
+    const int w = threadIdx.x & 15;
+    Acc a = acc_empty();
+    if (w * 64 < (int)blockDim.x) a = lds[w];
+    acc_rebase<ENT, NEAR>(a, lane_value(row_max(a.m), 0), c2);
+    a.s = lane_value(row_sum(a.s), 0);
+    if (ENT) a.e = lane_value(row_sum(a.e), 0);
+    a.n = lane_value(row_sum(a.n), 0);
+    return a;
+}
 
-template <typename T, int NT> struct Row {
-    static constexpr int N = VEC<T>;
-    u32x4 v[HELD];
-    T tail;
+// ------------------------------------------------------------------------------------------ who works on a row
+// A workgroup, or (WAVE) each of its four waves one row: rows of a few KB, for which a barrier would cost more than it
+// brings.
+struct Part {
+    int tid, nt, first;       // thread, threads, the wave's first thread (a scalar)
+};
+template <bool WAVE> __device__ __forceinline__ Part part_of() {
+    if (WAVE) return {(int)(threadIdx.x & 63), 64, 0};
+    return {(int)threadIdx.x, (int)blockDim.x, __builtin_amdgcn_readfirstlane(threadIdx.x) & ~63};
+}
+// A row cut at the 16-byte boundaries of its logits: rows of an odd vocabulary begin anywhere, and reading them in
+// 16-byte steps from there was measured at 4.9 TB/s against 6.1 for aligned steps.  The logits before the first and
+// behind the last boundary, up to 7 at either end, are the edge: one scalar of threads 0-6 and 8-14.
+template <typename T> struct Span {
+    int V, head, nvec;
 
-    __device__ __forceinline__ void load(const T* x, int V) {
-        const int nvec = V / N;
-#pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            v[i] = Word<T>::LOWEST;
-            if ((int)threadIdx.x < nvec - i * NT) v[i] = load_at(x + i * NT * N);
-        }
-        tail = (T)-__builtin_inff();
-        if ((int)threadIdx.x < V - nvec * N) tail = x[nvec * N + threadIdx.x];
+    __device__ __forceinline__ Span(const T* x, int V) : V(V) {
+        head = min(V, (int)(-(uintptr_t)x % 16u / sizeof(T)));
+        nvec = (V - head) / VEC<T>;
+    }
+    __device__ __forceinline__ int edge(int tid) const {      // this thread's logit of the edge, or -1
+        const int behind = head + nvec * VEC<T> + tid - 8;
+        return tid < 8 ? (tid < head ? tid : -1) : (tid < 16 && behind < V ? behind : -1);
     }
 };
 
-// vectors joined before each rescaling
-template <typename T> struct Step { static constexpr int M = sizeof(T) == 4 ? 4 : 2; };
+// vector j of the body; the gradient's may lie across a boundary
+template <typename T> __device__ __forceinline__ u32x4 load_vec(const T* body, int j) {
+    return *(const u32x4*)((const char*)body + 16u * (uint32_t)j);
+}
+template <typename T> __device__ __forceinline__ void store_vec(T* body, int j, u32x4 o) {
+    __builtin_memcpy((char*)body + 16u * (uint32_t)j, &o, 16);
+}
 
-template <typename T, int NT, bool ENT>
-__device__ __forceinline__ Acc row_stats(const Row<T, NT>& row, const T* x, int V, float c2, Acc* lds) {
-    constexpr int N = VEC<T>, M = Step<T>::M;
-    const int nvec = V / N;
+// (m, S, E) of a row that is not kept, joined over the wave.  STREAM vectors of a thread are on their way while the
+// STREAM before are added.
+#define STREAM 4
+template <typename T, bool ENT, bool NEAR>
+__device__ __forceinline__ Acc stream_stats(const T* x, int V, float c2, const Part p, float counted) {
+    constexpr int N = VEC<T>;
+    const Span<T> s(x, V);
+    const T* body = x + s.head;
+    const int e = s.edge(p.tid);
+    const float edge = e >= 0 ? wide(x[e]) : -__builtin_inff();
     Acc a = acc_empty();
+    a.n = counted;
+    if (s.nvec > 0) {
+        const int step = STREAM * p.nt, steps = s.nvec / step, left = s.nvec - steps * step;
+        u32x4 v[STREAM], next[STREAM];
+        const T* from = body;
+        auto fetch = [&]() {          // a step of which every thread has its part
 #pragma unroll
-    for (int i = 0; i < HELD; i += M) {
-        if (i * NT >= nvec) break;
-        acc_vecs<T, M, ENT>(a, row.v + i, c2);
+            for (int k = 0; k < STREAM; ++k) next[k] = load_vec(from + (int64_t)k * p.nt * N, p.tid);
+        };
+        if (steps > 0) fetch();
+        for (int i = 1; i < steps; ++i) {
+            from += (int64_t)step * N;
+#pragma unroll
+            for (int k = 0; k < STREAM; ++k) v[k] = next[k];
+            fetch();
+            __builtin_amdgcn_sched_barrier(0);    // the loads stay ahead of the arithmetic
+            acc_vecs<T, STREAM, ENT, NEAR>(a, v, c2);
+        }
+        if (steps > 0) {
+#pragma unroll
+            for (int k = 0; k < STREAM; ++k) v[k] = next[k];
+        }
+        // the last step, which may be empty: threads without a part read the last vector of the row
+#pragma unroll
+        for (int k = 0; k < STREAM; ++k) next[k] = load_vec(body, min(steps * step + k * p.nt + p.tid, s.nvec - 1));
+        __builtin_amdgcn_sched_barrier(0);
+        if (steps > 0) acc_vecs<T, STREAM, ENT, NEAR>(a, v, c2);
+#pragma unroll
+        for (int k = 0; k < STREAM; ++k)
+            if (k * p.nt + p.first < left) {      // some lane of this wave has a part
+                if (k * p.nt + p.tid >= left) next[k] = Word<T>::LOWEST;
+                acc_vecs<T, 1, ENT, NEAR>(a, next + k, c2);
+            }
     }
-    if (NT == 1024)
-        for (int j = HELD * NT + threadIdx.x; j < nvec; j += NT) {
-            const u32x4 v = load_vec(x + (int64_t)j * N);
+    acc_rebase<ENT, NEAR>(a, fmaxf(a.m, edge), c2);
+    acc_add<ENT, NEAR>(a, edge, c2);
+    return acc_wave<ENT, NEAR>(a, c2);
+}
+
+// The same joined over the workgroup in its first wave: true there, and the other waves are done.
+template <typename T, bool WAVE, bool ENT>
+__device__ __forceinline__ bool stream_row(const T* x, int V, float c2, float counted, Acc* lds, Acc& a) {
+    a = stream_stats<T, ENT, true>(x, V, c2, part_of<WAVE>(), counted);
+    if (!WAVE) {
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
+        __syncthreads();
+        if (threadIdx.x >= 64) return false;
+        a = acc_waves<ENT, true>(lds, c2);
+    }
+    const float n = a.n;
+    if (is_near(a.m, c2)) a = near_done(a, c2);
+    else a = stream_stats<T, ENT, false>(x, V, c2, part_of<true>(), 0.0f);
+    a.n = n;
+    return true;
+}
+
+// ------------------------------------------------------------------------------------------ a row on the chip
+// A row's threads hold CH vectors each, so that statistics and gradient read memory once: 16 threads of vectors a
+// lane are 64 registers, 1024 threads then hold 256 KB.  Vectors beyond are read again for the gradient.  Vector j
+// belongs to thread j % nt; lanes past the end of the row hold its last vector, which is not counted or stored.
+template <typename T, int CH> struct Row {
+    u32x4 v[CH];
+    float edge;
+};
+
+template <typename T, int CH>
+__device__ __forceinline__ void row_load(Row<T, CH>& row, const T* x, const Span<T>& s, const Part& p) {
+    const int e = s.edge(p.tid);
+    row.edge = e >= 0 ? wide(x[e]) : -__builtin_inff();
+    if (s.nvec > 0) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) row.v[i] = load_vec(x + s.head, min(i * p.nt + p.tid, s.nvec - 1));
+    }
+}
+
+template <typename T, int CH, bool WAVE, bool ENT>
+__device__ __forceinline__ Acc row_stats(Row<T, CH>& row, const T* x, const Span<T>& s, const Part& p, float c2,
+                                         float counted, Acc* lds) {
+    constexpr int M = sizeof(T) == 4 ? 4 : 2;             // vectors added at once
+    const int mine = s.nvec - p.first;
+    Acc a = acc_empty();
+    a.n = counted;
+#pragma unroll
+    for (int i = 0; i < CH; i += M) {
+        if (i * p.nt < mine) {
+#pragma unroll
+            for (int k = i; k < i + M; ++k)
+                if (k * p.nt + 64 > mine && k * p.nt + p.tid >= s.nvec) row.v[k] = Word<T>::LOWEST;
+            acc_vecs<T, M, ENT>(a, row.v + i, c2);
+        }
+    }
+    if (CH == 16)
+        for (int j = CH * p.nt + p.tid; j < s.nvec; j += p.nt) {
+            const u32x4 v = load_vec(x + s.head, j);
             acc_vecs<T, 1, ENT>(a, &v, c2);
         }
-    const float t = wide(row.tail);
-    acc_rebase<ENT>(a, fmaxf(a.m, t), c2);
-    acc_add<ENT>(a, t, c2);
-    return acc_block<NT, ENT>(a, c2, lds);
+    acc_rebase<ENT>(a, fmaxf(a.m, row.edge), c2);
+    acc_add<ENT>(a, row.edge, c2);
+    a = acc_wave<ENT>(a, c2);
+    if (WAVE) return a;
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
+    __syncthreads();
+    return acc_waves<ENT>(lds, c2);
 }
 
 // ------------------------------------------------------------------------------------------ row gradient
@@ -253,61 +356,68 @@ template <bool ENT> __device__ __forceinline__ float grad_of(const RowGrad& g, f
 }
 
 template <typename T, bool ENT>
-__device__ __forceinline__ u32x4 grad_vec(const RowGrad& g, u32x4 v, int j, float c2) {
+__device__ __forceinline__ u32x4 grad_vec(const RowGrad& g, u32x4 v, int place, float c2) {   // place: of the token in v
     constexpr int N = VEC<T>;
     float d[N];
     unpack<T>(v, d);
 #pragma unroll
     for (int i = 0; i < N; ++i) d[i] = grad_of<ENT>(g, d[i], c2);
-    if (j == g.tok / N && g.tok >= 0) {
+    if (place >= 0 && place < N) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) d[i] += i == g.tok % N ? g.gt : 0.0f;
+        for (int i = 0; i < N; ++i) d[i] += i == place ? g.gt : 0.0f;
     }
     return pack<T>(d);        // the one rounding of the gradient
 }
 
-template <typename T, bool ENT> __device__ __forceinline__ T grad_one(const RowGrad& g, T x, int i, float c2) {
-    const float d = grad_of<ENT>(g, wide(x), c2);
-    return (T)(i == g.tok ? d + g.gt : d);
+template <typename T, bool ENT>
+__device__ __forceinline__ void edge_grad(const RowGrad& g, float x, T* out, int i, float c2) {
+    if (i < 0) return;
+    const float d = grad_of<ENT>(g, x, c2);
+    out[i] = (T)(i == g.tok ? d + g.gt : d);
 }
 
-// the gradient of a held row; the vectors that are read again may lie where the gradient goes
-template <typename T, int NT, bool ENT>
-__device__ __forceinline__ void row_grad(const Row<T, NT>& row, const T* x, T* out, int V, float c2, const RowGrad& g) {
+// The gradient of a held row.  The vectors that are read again may lie where their gradient goes.
+template <typename T, int CH, bool ENT>
+__device__ __forceinline__ void row_grad(const Row<T, CH>& row, const T* x, T* out, const Span<T>& s, const Part& p,
+                                         float c2, const RowGrad& g) {
     constexpr int N = VEC<T>;
-    const int nvec = V / N;
+    const int mine = s.nvec - p.first;
+    const int tok = g.tok >= 0 ? g.tok - s.head : -1;
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        if (i * NT >= nvec) break;
-        const u32x4 o = grad_vec<T, ENT>(g, row.v[i], i * NT + threadIdx.x, c2);
-        if ((int)threadIdx.x < nvec - i * NT) store_at(out + i * NT * N, o);
+    for (int i = 0; i < CH; ++i) {
+        if (i * p.nt < mine) {
+            const int j = i * p.nt + p.tid;
+            const u32x4 o = grad_vec<T, ENT>(g, row.v[i], tok - j * N, c2);
+            if (j < s.nvec) store_vec(out + s.head, j, o);
+        }
     }
-    if (NT == 1024)
-        for (int j = HELD * NT + threadIdx.x; j < nvec; j += NT)
-            store_vec(out + (int64_t)j * N, grad_vec<T, ENT>(g, load_vec(x + (int64_t)j * N), j, c2));
-    const int i = nvec * N + threadIdx.x;
-    if (i < V) out[i] = grad_one<T, ENT>(g, row.tail, i, c2);
+    if (CH == 16)
+        for (int j = CH * p.nt + p.tid; j < s.nvec; j += p.nt)
+            store_vec(out + s.head, j, grad_vec<T, ENT>(g, load_vec(x + s.head, j), tok - j * N, c2));
+    edge_grad<T, ENT>(g, row.edge, out, s.edge(p.tid), c2);
 }
 
-// the gradient of a row whose statistics are known; x may be out
-template <typename T, int NT, bool ENT>
-__device__ __forceinline__ void row_map(const T* x, T* out, int V, float c2, const RowGrad& g) {
+// The gradient of a row whose statistics are known, vectors j0 up to j1; x may be out.
+template <typename T, bool ENT>
+__device__ __forceinline__ void row_map(const T* x, T* out, int V, const Part& p, int seg, int segs, float c2,
+                                        const RowGrad& g) {
     constexpr int N = VEC<T>;
-    const int nvec = V / N;
-    for (int j = threadIdx.x; j < nvec; j += NT)
-        store_vec(out + (int64_t)j * N, grad_vec<T, ENT>(g, load_vec(x + (int64_t)j * N), j, c2));
-    for (int i = nvec * N + threadIdx.x; i < V; i += NT) out[i] = grad_one<T, ENT>(g, x[i], i, c2);
+    const Span<T> s(x, V);
+    const int per = (s.nvec + segs - 1) / segs, end = min(s.nvec, (seg + 1) * per);
+    const int tok = g.tok >= 0 ? g.tok - s.head : -1;
+    for (int j = seg * per + p.tid; j < end; j += p.nt)
+        store_vec(out + s.head, j, grad_vec<T, ENT>(g, load_vec(x + s.head, j), tok - j * N, c2));
+    const int e = seg == 0 ? s.edge(p.tid) : -1;
+    edge_grad<T, ENT>(g, e >= 0 ? wide(x[e]) : 0.0f, out, e, c2);
 }
 
-template <typename T, int NT> __device__ __forceinline__ void row_fill(T* out, int V, float value) {
-    constexpr int N = VEC<T>;
-    const int nvec = V / N;
-    float f[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = value;
-    const u32x4 o = pack<T>(f);
-    for (int j = threadIdx.x; j < nvec; j += NT) store_vec(out + (int64_t)j * N, o);
-    for (int i = nvec * N + threadIdx.x; i < V; i += NT) out[i] = (T)value;
+template <typename T> __device__ __forceinline__ void row_fill(T* out, int V, const Part& p, int seg = 0, int segs = 1) {
+    const Span<T> s(out, V);
+    const int per = (s.nvec + segs - 1) / segs, end = min(s.nvec, (seg + 1) * per);
+    const u32x4 zero = 0;
+    for (int j = seg * per + p.tid; j < end; j += p.nt) store_vec(out + s.head, j, zero);
+    const int e = seg == 0 ? s.edge(p.tid) : -1;
+    if (e >= 0) out[e] = (T)0.0f;
 }
 
 // ------------------------------------------------------------------------------------------ launch arguments
@@ -316,31 +426,65 @@ struct Logits {
     void* grad;               // may be x itself
     int64_t xs, xt, gs, gt;   // strides (elements) of sequences and tokens
     int64_t n_tok, n;         // n = sequences * n_tok rows
+    int64_t r0;               // first row of this launch
     int V;
     float c, c2;              // 1/temperature; the same times log2(e)
 };
 
-template <typename T> __device__ __forceinline__ const T* row_in(const Logits& L, int64_t b, int64_t t) {
-    return (const T*)L.x + b * L.xs + t * L.xt;
+template <bool WAVE> __device__ __forceinline__ int64_t row_of(const Logits& L) {
+    return L.r0 + (WAVE ? (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : (int64_t)blockIdx.x);
 }
-template <typename T> __device__ __forceinline__ T* row_out(const Logits& L, int64_t b, int64_t t) {
-    return (T*)L.grad + b * L.gs + t * L.gt;
+
+struct Place {
+    uint32_t b, t;            // sequence and position
+};
+__device__ __forceinline__ Place place_of(const Logits& L, int64_t r) {   // rows are fewer than 2^31: one 32-bit division
+    const uint32_t b = (uint32_t)r / (uint32_t)L.n_tok;
+    return {b, (uint32_t)r - b * (uint32_t)L.n_tok};
+}
+
+template <typename T> __device__ __forceinline__ const T* row_in(const Logits& L, const Place& at) {
+    return (const T*)L.x + (int64_t)at.b * L.xs + (int64_t)at.t * L.xt;
+}
+template <typename T> __device__ __forceinline__ T* row_out(const Logits& L, const Place& at) {
+    return (T*)L.grad + (int64_t)at.b * L.gs + (int64_t)at.t * L.gt;
 }
 
 struct Weights {              // how much a row counts
     const uint8_t* mask;      // NULL: every row counts
-    const int* seq_len;       // counted rows of each sequence (masks only)
-    const int* totals;        // {counted rows, sequences with one} (masks only)
+    const int* seq_len;       // counted rows of each sequence
+    const int* totals;        // {counted rows, sequences with one}
     int reduction;
+    int count_here;           // each row's threads count the whole mask themselves
     float scale;
     int64_t n_seq;
 };
 
-__device__ __forceinline__ float row_weight(const Weights& w, int64_t b, int64_t n_tok) {   // of a counted row
+#define COUNT_HERE 4096       // rows up to which that is cheaper than a launch (16 bytes of the mask are one load)
+
+// This thread's part of the counted rows.
+__device__ __forceinline__ float count_mask(const Weights& w, int64_t n, const Part& p) {
+    int k = 0;
+    if (w.count_here) {
+        const int whole = (int)n / 16;
+        for (int j = p.tid; j < whole; j += p.nt) {
+            u32x4 v;
+            __builtin_memcpy(&v, w.mask + 16 * j, 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)   // bytes that are not 0
+                k += __popc((((v[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | v[i]) & 0x80808080u);
+        }
+        const int j = whole * 16 + p.tid;
+        if (p.tid < 16 && j < (int)n) k += w.mask[j] != 0;
+    }
+    return (float)k;          // below 2^24 in any sum: exact
+}
+
+__device__ __forceinline__ float row_weight(const Weights& w, const Place& at, int64_t n_tok, float counted) {
     double d = 1.0;
-    if (w.reduction == RED_TOKEN) d = w.mask ? (double)w.totals[0] : (double)w.n_seq * (double)n_tok;
-    if (w.reduction == RED_SEQ)
-        d = w.mask ? (double)w.seq_len[b] * (double)w.totals[1] : (double)w.n_seq * (double)n_tok;
+    if (w.reduction != RED_SUM && !w.mask) d = (double)w.n_seq * (double)n_tok;
+    else if (w.reduction == RED_TOKEN) d = w.count_here ? (double)counted : (double)w.totals[0];
+    else if (w.reduction == RED_SEQ) d = (double)w.seq_len[at.b] * (double)w.totals[1];
     return (float)((double)w.scale / d);
 }
 
@@ -363,11 +507,15 @@ __device__ __forceinline__ double ln_of(float s) {
     return fma((double)k, LN2_D, 2.0 * z * p);
 }
 
-// log-probability of `tok`, NaN for one that is not in the vocabulary (its row of logits is not indexed with it)
-template <typename T>
-__device__ __forceinline__ double token_logp(const T* x, int64_t tok, int V, float c, const Acc& a, double ln_s) {
-    if (tok < 0 || tok >= V) return __builtin_nan("");
-    return ((double)wide(x[tok]) - (double)a.m) * (double)c - ln_s;
+// The token's logit, NaN for a token that is not in the vocabulary.
+template <typename T> __device__ __forceinline__ float token_logit(const T* x, int64_t tok, int V) {
+    return tok >= 0 && tok < V ? wide(x[tok]) : __builtin_nanf("");
+}
+__device__ __forceinline__ double logp_of(float x, float c, const Acc& a, double ln_s) {
+    return ((double)x - (double)a.m) * (double)c - ln_s;
+}
+__device__ __forceinline__ float entropy_of(const Acc& a, double ln_s) {
+    return (float)(ln_s - LN2_D * (double)(a.e / a.s));
 }
 
 // ------------------------------------------------------------------------------------------ counting masks
@@ -411,48 +559,49 @@ __global__ __launch_bounds__(1024) void count_kernel(const uint8_t* __restrict__
     }
 }
 
-// sum of `n` partial losses in a fixed order
-__global__ __launch_bounds__(1024) void total_kernel(const double* __restrict__ part, int n, float* loss) {
+// The rows' losses summed in a fixed order.  One workgroup, or (loss == NULL) one of several that leave their sums for
+// a second launch.
+__global__ __launch_bounds__(1024) void total_kernel(const double* __restrict__ part, int64_t n, double* sums, float* loss) {
     __shared__ double lds[16];
     double s = 0.0;
-    for (int i = threadIdx.x; i < n; i += 1024) s += part[i];
+    for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 1024) s += part[i];
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 16; ++w) s += lds[w];
-        *loss = (float)s;
+        if (loss) *loss = (float)s;
+        else sums[blockIdx.x] = s;
     }
 }
 
 // ------------------------------------------------------------------------------------------ log-probabilities
-template <typename T, int NT, bool ENT>
-__global__ __launch_bounds__(NT, 4) void logprobs_kernel(Logits L, const void* tokens, int i64, const uint8_t* mask,
-                                                      float* logprobs, double* logprobs64, float* entropy,
-                                                      RowStats* stats) {
-    __shared__ Acc lds[NT / 64];
-    for (int64_t r = blockIdx.x; r < L.n; r += gridDim.x) {
-        const int64_t b = r / L.n_tok, t = r - b * L.n_tok;
-        double lp = 0.0;
-        RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
-        if (!mask || mask[r]) {
-            const T* x = row_in<T>(L, b, t);
-            Row<T, NT> row;
-            row.load(x, L.V);
-            const Acc a = row_stats<T, NT, ENT>(row, x, L.V, L.c2, lds);
-            const double ln_s = ln_of(a.s);
-            lp = token_logp(x, int_at(tokens, i64, r), L.V, L.c, a, ln_s);
-            st.m = a.m;
-            st.s = a.s;
-            if (ENT) st.h = (float)(ln_s - LN2_D * (double)(a.e / a.s));
-        }
-        if (threadIdx.x == 0) {
-            if (logprobs) logprobs[r] = (float)lp;
-            if (logprobs64) logprobs64[r] = lp;
-            if (ENT && entropy) entropy[r] = st.h;
-            if (stats) stats[r] = st;
-        }
+template <typename T, bool WAVE, bool ENT>
+__global__ __launch_bounds__(1024, 4) void logprobs_kernel(Logits L, const void* tokens, int i64, const uint8_t* mask,
+                                                           float* logprobs, double* logprobs64, float* entropy,
+                                                           RowStats* stats) {
+    __shared__ Acc lds[16];
+    const int64_t r = row_of<WAVE>(L);
+    if (WAVE && r >= L.n) return;
+    double lp = 0.0;
+    RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
+    if (!mask || mask[r]) {
+        const T* x = row_in<T>(L, place_of(L, r));
+        const float xt = token_logit(x, int_at(tokens, i64, r), L.V);
+        Acc a;
+        if (!stream_row<T, WAVE, ENT>(x, L.V, L.c2, 0.0f, lds, a)) return;
+        const double ln_s = ln_of(a.s);
+        lp = logp_of(xt, L.c, a, ln_s);
+        st.m = a.m;
+        st.s = a.s;
+        if (ENT) st.h = entropy_of(a, ln_s);
+    }
+    if (part_of<WAVE>().tid == 0) {
+        if (logprobs) logprobs[r] = (float)lp;
+        if (logprobs64) logprobs64[r] = lp;
+        if (ENT && entropy) entropy[r] = st.h;
+        if (stats) stats[r] = st;
     }
 }
 
@@ -474,23 +623,24 @@ struct Incoming {             // dL/dlogp and dL/dH of each row, and a factor on
     int64_t lp_s, lp_t, h_s, h_t;
 };
 
-template <typename T, int NT, bool ENT>
-__global__ __launch_bounds__(NT, 4) void backward_kernel(Logits L, const void* tokens, int i64, const uint8_t* mask,
-                                                      const RowStats* __restrict__ stats, Incoming in) {
-    const float f = in.factor ? *in.factor : 1.0f;
-    for (int64_t r = blockIdx.x; r < L.n; r += gridDim.x) {
-        const int64_t b = r / L.n_tok, t = r - b * L.n_tok;
-        T* out = row_out<T>(L, b, t);
-        if (mask && !mask[r]) {
-            row_fill<T, NT>(out, L.V, 0.0f);
-            continue;
-        }
-        const RowStats st = stats[r];
-        const float g_lp = in.lp ? f * in.lp[b * in.lp_s + t * in.lp_t] : 0.0f;
-        const float g_h = ENT ? f * in.h[b * in.h_s + t * in.h_t] : 0.0f;
-        const RowGrad g = grad_seed(st.m, st.s, st.h, g_lp, g_h, int_at(tokens, i64, r), L.V, L.c);
-        row_map<T, NT, ENT>(row_in<T>(L, b, t), out, L.V, L.c2, g);
+template <typename T, bool WAVE, bool ENT>
+__global__ __launch_bounds__(256) void backward_kernel(Logits L, const void* tokens, int i64, const uint8_t* mask,
+                                                       const RowStats* __restrict__ stats, Incoming in) {
+    const int64_t r = row_of<WAVE>(L);
+    if (WAVE && r >= L.n) return;
+    const Part p = part_of<WAVE>();
+    const Place at = place_of(L, r);
+    T* out = row_out<T>(L, at);
+    if (mask && !mask[r]) {
+        row_fill(out, L.V, p, blockIdx.y, gridDim.y);
+        return;
     }
+    const float f = in.factor ? *in.factor : 1.0f;
+    const RowStats st = stats[r];
+    const float g_lp = in.lp ? f * in.lp[at.b * in.lp_s + at.t * in.lp_t] : 0.0f;
+    const float g_h = ENT ? f * in.h[at.b * in.h_s + at.t * in.h_t] : 0.0f;
+    const RowGrad g = grad_seed(st.m, st.s, st.h, g_lp, g_h, int_at(tokens, i64, r), L.V, L.c);
+    row_map<T, ENT>(row_in<T>(L, at), out, L.V, p, blockIdx.y, gridDim.y, L.c2, g);
 }
 
 // ------------------------------------------------------------------------------------------ clipped policy loss
@@ -504,7 +654,7 @@ struct PolicyArgs {
     float *logprobs, *entropy;
     RowStats* stats;          // with seeds: the differentiable form
     float *g_lp, *g_h;
-    double* part;
+    double* part;             // weighted loss of each row
 };
 
 struct PolicyRow {
@@ -535,48 +685,90 @@ __device__ __forceinline__ PolicyRow policy_row(const PolicyArgs& p, double lp, 
     return {loss * (double)w, w * g, -w * p.ent};
 }
 
-template <typename T, int NT, bool GRAD, bool ENT_GRAD>
-__global__ __launch_bounds__(NT, 4) void policy_kernel(Logits L, PolicyArgs p) {
-    __shared__ Acc lds[NT / 64];
-    double total = 0.0;
-    for (int64_t r = blockIdx.x; r < L.n; r += gridDim.x) {
-        const int64_t b = r / L.n_tok, t = r - b * L.n_tok;
-        RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
-        double lp = 0.0;
-        PolicyRow o = {0.0, 0.0f, 0.0f};
-        if (!p.w.mask || p.w.mask[r]) {
-            const T* x = row_in<T>(L, b, t);
-            Row<T, NT> row;
-            row.load(x, L.V);
-            const Acc a = row_stats<T, NT, true>(row, x, L.V, L.c2, lds);
-            const double ln_s = ln_of(a.s);
-            const int64_t tok = int_at(p.tokens, p.i64, r);
-            lp = token_logp(x, tok, L.V, L.c, a, ln_s);
-            st.m = a.m;
-            st.s = a.s;
-            st.h = (float)(ln_s - LN2_D * (double)(a.e / a.s));
-            o = policy_row(p, lp, st.h, p.old_lp[r], p.adv[b * p.adv_s + t * p.adv_t], p.ref ? p.ref[r] : 0.0f,
-                           row_weight(p.w, b, L.n_tok));
-            total += o.loss;
-            if (GRAD) {
-                __syncthreads();   // x[tok] has been read by all: the gradient may overwrite the logits
-                row_grad<T, NT, ENT_GRAD>(row, x, row_out<T>(L, b, t), L.V, L.c2,
-                                          grad_seed(a.m, a.s, st.h, o.g_lp, o.g_h, tok, L.V, L.c));
-            }
-        } else if (GRAD) {
-            row_fill<T, NT>(row_out<T>(L, b, t), L.V, 0.0f);
-        }
-        if (threadIdx.x == 0) {
-            if (p.logprobs) p.logprobs[r] = (float)lp;
-            if (p.entropy) p.entropy[r] = st.h;
-            if (!GRAD && p.stats) {
-                p.stats[r] = st;
-                p.g_lp[r] = o.g_lp;
-                p.g_h[r] = o.g_h;
-            }
-        }
+// inputs of a counted row
+struct PolicyIn {
+    float xt, old_lp, adv, ref;
+    int64_t tok;
+};
+template <typename T>
+__device__ __forceinline__ PolicyIn policy_in(const Logits& L, const PolicyArgs& p, const T* x, int64_t r, const Place& at) {
+    PolicyIn i;
+    i.tok = int_at(p.tokens, p.i64, r);
+    i.old_lp = p.old_lp[r];
+    i.adv = p.adv[at.b * p.adv_s + at.t * p.adv_t];
+    i.ref = p.ref ? p.ref[r] : 0.0f;
+    i.xt = token_logit(x, i.tok, L.V);
+    return i;
+}
+
+// Forward only; leaves what the backward pass needs.
+template <typename T, bool WAVE>
+__global__ __launch_bounds__(1024, 4) void policy_forward_kernel(Logits L, PolicyArgs p) {
+    __shared__ Acc lds[16];
+    const int64_t r = row_of<WAVE>(L);
+    if (WAVE && r >= L.n) return;
+    RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
+    double lp = 0.0;
+    PolicyRow o = {0.0, 0.0f, 0.0f};
+    if (!p.w.mask || p.w.mask[r]) {
+        const Place at = place_of(L, r);
+        const T* x = row_in<T>(L, at);
+        const PolicyIn in = policy_in(L, p, x, r, at);
+        Acc a;
+        if (!stream_row<T, WAVE, true>(x, L.V, L.c2, count_mask(p.w, L.n, part_of<WAVE>()), lds, a)) return;
+        const double ln_s = ln_of(a.s);
+        lp = logp_of(in.xt, L.c, a, ln_s);
+        st.m = a.m;
+        st.s = a.s;
+        st.h = entropy_of(a, ln_s);
+        o = policy_row(p, lp, st.h, in.old_lp, in.adv, in.ref, row_weight(p.w, at, L.n_tok, a.n));
     }
-    if (threadIdx.x == 0) p.part[blockIdx.x] = total;
+    if (part_of<WAVE>().tid == 0) {
+        p.logprobs[r] = (float)lp;
+        if (p.entropy) p.entropy[r] = st.h;
+        if (p.stats) {
+            p.stats[r] = st;
+            p.g_lp[r] = o.g_lp;
+            p.g_h[r] = o.g_h;
+        }
+        p.part[r] = o.loss;
+    }
+}
+
+// Loss and gradient: the row stays on the chip between its statistics and its gradient.
+template <typename T, int CH, bool WAVE, bool ENT_GRAD>
+__global__ __launch_bounds__(WAVE ? 256 : 1024, 4) void policy_kernel(Logits L, PolicyArgs p) {
+    __shared__ Acc lds[16];
+    const int64_t r = row_of<WAVE>(L);
+    if (WAVE && r >= L.n) return;
+    const Part q = part_of<WAVE>();
+    const Place at = place_of(L, r);
+    T* out = row_out<T>(L, at);
+    double lp = 0.0, loss = 0.0;
+    float h = 0.0f;
+    if (!p.w.mask || p.w.mask[r]) {
+        const T* x = row_in<T>(L, at);
+        const Span<T> s(x, L.V);
+        Row<T, CH> row;
+        const PolicyIn in = policy_in(L, p, x, r, at);
+        row_load(row, x, s, q);
+        const float counted = count_mask(p.w, L.n, q);
+        asm volatile("" :: "v"(in.xt));   // read before the barrier in row_stats: the gradient may overwrite it
+        const Acc a = row_stats<T, CH, WAVE, true>(row, x, s, q, L.c2, counted, lds);
+        const double ln_s = ln_of(a.s);
+        lp = logp_of(in.xt, L.c, a, ln_s);
+        h = entropy_of(a, ln_s);
+        const PolicyRow o = policy_row(p, lp, h, in.old_lp, in.adv, in.ref, row_weight(p.w, at, L.n_tok, a.n));
+        loss = o.loss;
+        row_grad<T, CH, ENT_GRAD>(row, x, out, s, q, L.c2, grad_seed(a.m, a.s, h, o.g_lp, o.g_h, in.tok, L.V, L.c));
+    } else {
+        row_fill(out, L.V, q);
+    }
+    if (q.tid == 0) {
+        p.logprobs[r] = (float)lp;
+        if (p.entropy) p.entropy[r] = h;
+        p.part[r] = loss;
+    }
 }
 
 // ------------------------------------------------------------------------------------------ preference loss
@@ -625,160 +817,171 @@ struct TeacherArgs {
     double* part;
 };
 
-struct Teacher {              // one row's entries, in LDS
-    int index[PPO_MAX_TEACHER_TOP];     // -1: padding
-    float q[PPO_MAX_TEACHER_TOP];       // teacher's probability of the entry
-    float all[PPO_MAX_TEACHER_TOP];     // the same summed over the entries of this index
-    float u[PPO_MAX_TEACHER_TOP];       // the student's logit there
-    float entropy, loss;                // sum q ln q; the row's loss
-    int bad, some;                      // a token beyond the vocabulary; an entry that is not padding
+// One row's entries, K of each array in LDS.  The first wave makes them while the others wait for their logits.
+struct Teacher {
+    int* index;               // -1: padding
+    float* q;                 // the teacher's probability of the entry
+    float* x;                 // the policy's logit there
+    int* bad;                 // a token beyond the vocabulary
+    int* some;                // an entry that is not padding
+    __device__ __forceinline__ Teacher(int* lds, int K)
+        : index(lds + 2), q((float*)(lds + 2 + K)), x((float*)(lds + 2 + 2 * K)), bad(lds), some(lds + 1) {}
 };
+static size_t teacher_lds(int K) { return (size_t)(2 + 3 * K) * 4; }
 
-// Reads the row's entries and makes them probabilities; two barriers at least lie before any of it is used.
-template <typename T, int NT>
-__device__ __forceinline__ void teacher_load(const TeacherArgs& p, const Logits& L, int64_t r, const T* x, Teacher& s) {
-    __syncthreads();          // the previous row's entries have been used
-    if (threadIdx.x == 0) s.bad = s.some = 0;
-    __syncthreads();
-    for (int k = threadIdx.x; k < p.K; k += NT) {
+// First wave only.  Returns sum q ln q.
+template <typename T>
+__device__ __forceinline__ float teacher_load(const TeacherArgs& p, const Logits& L, int64_t r, const T* x, const Teacher& s) {
+    const int lane = threadIdx.x;
+    float mx = -__FLT_MAX__, total = 0.0f, ent = 0.0f;
+    bool bad = false, some = false;
+    for (int k = lane; k < p.K; k += 64) {
         const int64_t i = int_at(p.index, p.i64, r * p.K + k);
+        const float t = float_at(p.logit, p.dtype, r * p.K + k);
         const bool there = i >= 0 && i < L.V;
-        if (i >= L.V) s.bad = 1;
-        if (there) s.some = 1;
+        bad |= i >= L.V;
+        some |= there;
         s.index[k] = there ? (int)i : -1;
-        s.q[k] = there ? float_at(p.logit, p.dtype, r * p.K + k) : 0.0f;
-        s.u[k] = there ? wide(x[i]) : 0.0f;
+        s.q[k] = t;
+        s.x[k] = there ? wide(x[i]) : 0.0f;
+        if (there) mx = fmaxf(mx, t);
     }
-    __syncthreads();
-    if (threadIdx.x < 64) {   // softmax over at most PPO_MAX_TEACHER_TOP entries: one wave
-        float mx = -__FLT_MAX__, total = 0.0f;
-        for (int k = threadIdx.x; k < p.K; k += 64)
-            if (s.index[k] >= 0) mx = fmaxf(mx, s.q[k]);
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
-        for (int k = threadIdx.x; k < p.K; k += 64) {
-            const float e = s.index[k] >= 0 ? expf((s.q[k] - mx) * L.c) : 0.0f;
-            s.all[k] = (s.q[k] - mx) * L.c;
-            s.q[k] = e;
-            total += e;
-        }
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) total += __shfl_xor(total, off);
-        float ent = 0.0f;     // sum q ln q
-        const float lt = (float)ln_of(total);
-        for (int k = threadIdx.x; k < p.K; k += 64) {
-            if (s.index[k] < 0) continue;
-            const float q = s.q[k] / total;
-            s.q[k] = q;
-            if (q != 0.0f) ent = fmaf(q, s.all[k] - lt, ent);
-        }
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) ent += __shfl_xor(ent, off);
-        if (threadIdx.x == 0) s.entropy = ent;
+    mx = wave_max(mx);
+    for (int k = lane; k < p.K; k += 64) total += s.index[k] >= 0 ? expf((s.q[k] - mx) * L.c) : 0.0f;
+    total = wave_sum(total);
+    const float lt = (float)ln_of(total);
+    for (int k = lane; k < p.K; k += 64) {
+        const float d = (s.q[k] - mx) * L.c, q = s.index[k] >= 0 ? expf(d) / total : 0.0f;
+        s.q[k] = q;
+        if (q != 0.0f) ent = fmaf(q, d - lt, ent);
     }
-    __syncthreads();
-    for (int k = threadIdx.x; k < p.K; k += NT) {
-        float all = 0.0f;
-        for (int j = 0; j < p.K; ++j) all += s.index[j] == s.index[k] ? s.q[j] : 0.0f;
-        s.all[k] = all;
+    bad = __any(bad);
+    some = __any(some);
+    if (lane == 0) {
+        *s.bad = bad;
+        *s.some = some;
     }
+    return wave_sum(ent);
 }
 
-// sum q (ln q - ln p), the same bits on every thread
-__device__ __forceinline__ float teacher_loss(const TeacherArgs& p, Teacher& s, float m, float c, double ln_s) {
-    __syncthreads();
-    if (threadIdx.x < 64) {
-        double cross = 0.0;
-        for (int k = threadIdx.x; k < p.K; k += 64)
-            if (s.index[k] >= 0 && s.q[k] != 0.0f)
-                cross += (double)s.q[k] * (((double)s.u[k] - (double)m) * (double)c - ln_s);
+// First wave only: sum q (ln q - ln p).
+__device__ __forceinline__ float teacher_loss(const TeacherArgs& p, const Teacher& s, float ent, const Acc& a, float c) {
+    const double ln_s = ln_of(a.s);
+    double cross = 0.0;
+    for (int k = threadIdx.x; k < p.K; k += 64)
+        if (s.q[k] != 0.0f) cross += (double)s.q[k] * logp_of(s.x[k], c, a, ln_s);
 #pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) cross += __shfl_xor(cross, off);
-        if (threadIdx.x == 0) s.loss = s.bad ? __builtin_nanf("") : (float)((double)s.entropy - cross);
-    }
-    __syncthreads();
-    return s.loss;
+    for (int off = 32; off >= 1; off >>= 1) cross += __shfl_xor(cross, off);
+    return *s.bad ? __builtin_nanf("") : (float)((double)ent - cross);
 }
 
 // dL/dx_i = g (p_i - sum of the teacher's q at i): the bulk first, the K places after a barrier.  A teacher that gave
 // nothing teaches nothing.
 __device__ __forceinline__ RowGrad teacher_seed(const Teacher& s, float m, float sum, float g) {
-    return {m, s.bad ? __builtin_nanf("") : s.some ? g / sum : 0.0f, 0.0f, 0.0f, -1};
+    return {m, *s.bad ? __builtin_nanf("") : *s.some ? g / sum : 0.0f, 0.0f, 0.0f, -1};
 }
 
-template <typename T, int NT>
+template <typename T>
 __device__ __forceinline__ void teacher_places(const TeacherArgs& p, const Teacher& s, T* out, const Logits& L,
                                                const RowGrad& rg, float g) {
     __syncthreads();          // the bulk is written
-    if (s.bad) return;
-    for (int k = threadIdx.x; k < p.K; k += NT)
-        if (s.index[k] >= 0) out[s.index[k]] = (T)(grad_of<false>(rg, s.u[k], L.c2) - g * s.all[k]);
+    if (*s.bad) return;
+    for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
+        const int i = s.index[k];
+        if (i < 0) continue;
+        float all = 0.0f;     // a token that appears twice: both entries, in both places the same number
+        for (int j = 0; j < p.K; ++j) all += s.index[j] == i ? s.q[j] : 0.0f;
+        out[i] = (T)(grad_of<false>(rg, s.x[k], L.c2) - g * all);
+    }
 }
 
-template <typename T, int NT, bool GRAD>
-__global__ __launch_bounds__(NT, 4) void distill_kernel(Logits L, TeacherArgs p) {
-    __shared__ Acc lds[NT / 64];
-    __shared__ Teacher teach;
-    const float temp = 1.0f / L.c;
-    double total = 0.0;
-    for (int64_t r = blockIdx.x; r < L.n; r += gridDim.x) {
-        const int64_t b = r / L.n_tok, t = r - b * L.n_tok;
-        RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
-        float loss = 0.0f;
-        if (!p.w.mask || p.w.mask[r]) {
-            const T* x = row_in<T>(L, b, t);
-            Row<T, NT> row;
-            row.load(x, L.V);
-            teacher_load<T, NT>(p, L, r, x, teach);
-            const Acc a = row_stats<T, NT, false>(row, x, L.V, L.c2, lds);
-            loss = temp * temp * teacher_loss(p, teach, a.m, L.c, ln_of(a.s));
-            st.m = a.m;
-            st.s = a.s;
-            st.w = row_weight(p.w, b, L.n_tok);
-            total += (double)st.w * (double)loss;
-            if (GRAD) {
-                T* out = row_out<T>(L, b, t);
-                const RowGrad g = teacher_seed(teach, a.m, a.s, st.w * temp);
-                row_grad<T, NT, false>(row, x, out, L.V, L.c2, g);
-                teacher_places<T, NT>(p, teach, out, L, g, st.w * temp);
-            }
-        } else if (GRAD) {
-            row_fill<T, NT>(row_out<T>(L, b, t), L.V, 0.0f);
-        }
-        if (threadIdx.x == 0) {
-            if (p.losses) p.losses[r] = loss;
-            if (!GRAD && p.stats) p.stats[r] = st;
-        }
+template <typename T>
+__global__ __launch_bounds__(1024, 4) void distill_forward_kernel(Logits L, TeacherArgs p) {
+    __shared__ Acc lds[16];
+    extern __shared__ int entries[];
+    const Teacher teach(entries, p.K);
+    const int64_t r = row_of<false>(L);
+    RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
+    float loss = 0.0f;
+    if (!p.w.mask || p.w.mask[r]) {
+        const Place at = place_of(L, r);
+        const T* x = row_in<T>(L, at);
+        float ent = 0.0f;
+        if (threadIdx.x < 64) ent = teacher_load(p, L, r, x, teach);
+        Acc a;
+        if (!stream_row<T, false, false>(x, L.V, L.c2, count_mask(p.w, L.n, part_of<false>()), lds, a)) return;
+        loss = teacher_loss(p, teach, ent, a, L.c) / (L.c * L.c);
+        st.m = a.m;
+        st.s = a.s;
+        st.w = row_weight(p.w, at, L.n_tok, a.n);
     }
-    if (threadIdx.x == 0) p.part[blockIdx.x] = total;
+    if (threadIdx.x == 0) {
+        if (p.losses) p.losses[r] = loss;
+        if (p.stats) p.stats[r] = st;
+        p.part[r] = (double)st.w * (double)loss;
+    }
 }
 
-template <typename T, int NT>
-__global__ __launch_bounds__(NT, 4) void distill_backward_kernel(Logits L, TeacherArgs p) {
-    __shared__ Teacher teach;
-    const float f = (p.factor ? *p.factor : 1.0f) / L.c;
-    for (int64_t r = blockIdx.x; r < L.n; r += gridDim.x) {
-        const int64_t b = r / L.n_tok, t = r - b * L.n_tok;
-        T* out = row_out<T>(L, b, t);
-        if (p.w.mask && !p.w.mask[r]) {
-            row_fill<T, NT>(out, L.V, 0.0f);
-            continue;
-        }
-        const T* x = row_in<T>(L, b, t);
-        const RowStats st = p.stats[r];
-        teacher_load<T, NT>(p, L, r, x, teach);
-        __syncthreads();
-        const RowGrad g = teacher_seed(teach, st.m, st.s, f * st.w);
-        row_map<T, NT, false>(x, out, L.V, L.c2, g);
-        teacher_places<T, NT>(p, teach, out, L, g, f * st.w);
+template <typename T, int CH>
+__global__ __launch_bounds__(1024, 4) void distill_kernel(Logits L, TeacherArgs p) {
+    __shared__ Acc lds[16];
+    extern __shared__ int entries[];
+    const Teacher teach(entries, p.K);
+    const int64_t r = row_of<false>(L);
+    const Part q = part_of<false>();
+    const Place at = place_of(L, r);
+    T* out = row_out<T>(L, at);
+    float loss = 0.0f, w = 0.0f;
+    if (!p.w.mask || p.w.mask[r]) {
+        const T* x = row_in<T>(L, at);
+        const Span<T> s(x, L.V);
+        Row<T, CH> row;
+        row_load(row, x, s, q);
+        float ent = 0.0f;
+        if (q.first == 0) ent = teacher_load(p, L, r, x, teach);
+        const Acc a = row_stats<T, CH, false, false>(row, x, s, q, L.c2, count_mask(p.w, L.n, q), lds);
+        w = row_weight(p.w, at, L.n_tok, a.n);
+        const RowGrad g = teacher_seed(teach, a.m, a.s, w / L.c);
+        row_grad<T, CH, false>(row, x, out, s, q, L.c2, g);
+        teacher_places(p, teach, out, L, g, w / L.c);
+        if (q.first == 0) loss = teacher_loss(p, teach, ent, a, L.c) / (L.c * L.c);
+    } else {
+        row_fill(out, L.V, q);
     }
+    if (threadIdx.x == 0) {
+        if (p.losses) p.losses[r] = loss;
+        p.part[r] = (double)w * (double)loss;
+    }
+}
+
+template <typename T> __global__ __launch_bounds__(256) void distill_backward_kernel(Logits L, TeacherArgs p) {
+    extern __shared__ int entries[];
+    const Teacher teach(entries, p.K);
+    const int64_t r = row_of<false>(L);
+    const Part q = part_of<false>();
+    const Place at = place_of(L, r);
+    T* out = row_out<T>(L, at);
+    if (p.w.mask && !p.w.mask[r]) {
+        row_fill(out, L.V, q);
+        return;
+    }
+    const T* x = row_in<T>(L, at);
+    if (q.first == 0) teacher_load(p, L, r, x, teach);
+    __syncthreads();
+    const RowStats st = p.stats[r];
+    const float g = (p.factor ? *p.factor : 1.0f) * st.w / L.c;
+    const RowGrad rg = teacher_seed(teach, st.m, st.s, g);
+    row_map<T, false>(x, out, L.V, q, 0, 1, L.c2, rg);
+    teacher_places(p, teach, out, L, rg, g);
 }
 
 // ------------------------------------------------------------------------------------------ host side
 #define ALIGN256(n) (((size_t)(n) + 255) & ~(size_t)255)
 
+#define TOTAL_GRID 64
+
 struct Workspace {            // one call's scratch
-    double* part;             // MAX_GRID partial losses, or one for each pair
+    double *part, *sums;      // weighted loss of each row (or pair); TOTAL_GRID sums of them
     int *totals, *seq_len;
     double* lp64;             // the pairs' log-probabilities
     float* seeds;             // and their gradients
@@ -790,7 +993,8 @@ static Workspace carve(void* base, int64_t n_seq, int64_t n_tok) {
     Workspace w;
     char* p = (char*)base;
     auto take = [&](size_t bytes) { char* q = p; p += ALIGN256(bytes); return q; };
-    w.part = (double*)take(8 * (size_t)(n_seq > MAX_GRID ? n_seq : MAX_GRID));
+    w.part = (double*)take(8 * (size_t)(n_tok > 0 ? n_seq * n_tok : n_seq));
+    w.sums = (double*)take(8 * TOTAL_GRID);
     w.totals = (int*)take(8);
     w.seq_len = (int*)take(4 * (size_t)n_seq);
     w.lp64 = (double*)take(8 * (size_t)(n_seq * n_tok));
@@ -832,41 +1036,61 @@ static Logits logits_of(const ppo_token_logits* x, void* grad) {
     L.gt = x->grad_tok_stride;
     L.n_tok = x->n_tok;
     L.n = x->n_seq * x->n_tok;
+    L.r0 = 0;
     L.V = (int)x->vocab;
     L.c = x->inv_temperature;
     L.c2 = x->inv_temperature * LOG2E_F;
     return L;
 }
 
-static int grid_of(int64_t n) { return (int)(n < MAX_GRID ? n : MAX_GRID); }
-
 #define BY_TYPE(dtype, T, ...)                                                     \
     if ((dtype) == PPO_F32) { using T = float; __VA_ARGS__; }                      \
     else if ((dtype) == PPO_BF16) { using T = __bf16; __VA_ARGS__; }               \
     else { using T = _Float16; __VA_ARGS__; }
+#define BY_FLAG(flag, F, ...)                                                      \
+    if (flag) { constexpr bool F = true; __VA_ARGS__; }                            \
+    else { constexpr bool F = false; __VA_ARGS__; }
 
-// Threads of a row: as few as hold it (a row is then in flight as a whole, and the more rows a CU has under way, the
-// more of one's memory time hides another's arithmetic).
-static int threads_of(const Logits& L, int dtype) {
-    const int64_t bytes = (int64_t)L.V * (dtype == PPO_F32 ? 4 : 2);
-    int nt = 64;
-    while (nt < 1024 && (int64_t)nt * HELD * 16 < bytes) nt *= 2;
-    return nt;
+static int64_t row_bytes(const Logits& L, int dtype) { return (int64_t)L.V * (dtype == PPO_F32 ? 4 : 2); }
+
+// A wave takes a row of up to 4 KB by itself: its 64 lanes hold that in four vectors each.
+static bool by_wave(const Logits& L, int dtype) { return row_bytes(L, dtype) <= 4096; }
+
+// A launch takes LAUNCH_ROWS rows at most: a grid of 2^32 threads and more is refused.  Runs its arguments for each
+// launch with the rows' first in L.r0 and `grid` workgroups of a row, or of four (WAVE).
+#define LAUNCH_ROWS (1 << 21)
+#define EACH_LAUNCH(L, WAVE, grid, ...)                                            \
+    for (L.r0 = 0; L.r0 < L.n; L.r0 += LAUNCH_ROWS) {                              \
+        const int rows_ = (int)(L.n - L.r0 < LAUNCH_ROWS ? L.n - L.r0 : LAUNCH_ROWS); \
+        const int grid = WAVE ? (rows_ + 3) / 4 : rows_;                           \
+        __VA_ARGS__;                                                               \
+    }
+
+// Threads of a row that is only read: few, because what is done once a row costs each wave the same, and the chip is
+// full with 256 rows under way and more; all that a workgroup can have where there are fewer rows than that.
+static int stream_threads(const Logits& L) { return L.n >= 512 ? 256 : 1024; }
+
+// Threads of a row that is held in CH vectors each: as many as it needs.
+static int held_threads(const Logits& L, int dtype, int CH) {
+    const int64_t waves = (row_bytes(L, dtype) + (int64_t)CH * 16 * 64 - 1) / ((int64_t)CH * 16 * 64);
+    return (int)(waves < 16 ? waves : 16) * 64;
+}
+// 8 vectors where 1024 threads hold the row so, else 16 (and the rest of a row beyond 256 KB is read twice)
+static bool held_in_8(const Logits& L, int dtype) { return row_bytes(L, dtype) <= 8 * 16 * 1024; }
+
+static void launch_total(const Workspace& w, int64_t n, float* loss, hipStream_t st) {
+    if (n <= 16384) {
+        total_kernel<<<1, 1024, 0, st>>>(w.part, n, nullptr, loss);
+        return;
+    }
+    total_kernel<<<TOTAL_GRID, 1024, 0, st>>>(w.part, n, w.sums, nullptr);
+    total_kernel<<<1, 1024, 0, st>>>(w.sums, TOTAL_GRID, nullptr, loss);
 }
 
-#define BY_THREADS(threads, NT, ...)                                               \
-    switch (threads) {                                                             \
-        case 64: { constexpr int NT = 64; __VA_ARGS__; break; }                    \
-        case 128: { constexpr int NT = 128; __VA_ARGS__; break; }                  \
-        case 256: { constexpr int NT = 256; __VA_ARGS__; break; }                  \
-        case 512: { constexpr int NT = 512; __VA_ARGS__; break; }                  \
-        default: { constexpr int NT = 1024; __VA_ARGS__; break; }                  \
-    }
-#define BY_TYPE_AND_THREADS(dtype, threads, T, NT, ...) BY_TYPE(dtype, T, BY_THREADS(threads, NT, __VA_ARGS__))
-
 // Counted rows of each sequence and of all, where a weight needs them.
-static void count_rows(const uint8_t* mask, int reduction, const ppo_token_logits* x, const Workspace& w, hipStream_t st) {
-    if (!mask || reduction == RED_SUM || x->n_seq * x->n_tok == 0) return;
+static void count_rows(const Weights& o, const ppo_token_logits* x, const Workspace& w, hipStream_t st) {
+    const uint8_t* mask = o.mask;
+    if (!mask || o.reduction == RED_SUM || o.count_here) return;
     if (x->n_seq * x->n_tok <= 32768) {
         count_kernel<<<1, 1024, 0, st>>>(mask, x->n_seq, x->n_tok, w.seq_len, w.totals, 1, 1);
         return;
@@ -879,33 +1103,43 @@ static void count_rows(const uint8_t* mask, int reduction, const ppo_token_logit
 static int weights_of(Weights* o, const uint8_t* mask, int reduction, float scale, const ppo_token_logits* x,
                       const Workspace& w) {
     if (reduction != RED_SUM && reduction != RED_TOKEN && reduction != RED_SEQ) return PPO_E_BADARG;
-    *o = {mask, w.seq_len, w.totals, reduction, scale, x->n_seq};
+    const int here = mask && reduction == RED_TOKEN && x->n_seq * x->n_tok <= COUNT_HERE;
+    *o = {mask, w.seq_len, w.totals, reduction, here, scale, x->n_seq};
     return 0;
+}
+
+static void launch_logprobs(Logits L, int dtype, const void* tokens, int i64, const uint8_t* mask, float* logprobs,
+                            double* logprobs64, float* entropy, RowStats* stats, hipStream_t st) {
+    BY_TYPE(dtype, T, BY_FLAG(by_wave(L, dtype), WAVE, BY_FLAG(entropy != nullptr, ENT, {
+        EACH_LAUNCH(L, WAVE, grid, (logprobs_kernel<T, WAVE, ENT><<<grid, WAVE ? 256 : stream_threads(L), 0, st>>>(
+            L, tokens, i64, mask, logprobs, logprobs64, entropy, stats)))
+    })))
+}
+
+// Parts of a row that the backward pass gives to a workgroup each, so that few rows fill the chip too: at least 16 KB.
+static int backward_parts(const Logits& L, int dtype) {
+    const int64_t want = (1024 + L.n - 1) / L.n, most = (row_bytes(L, dtype) + 16383) / 16384;
+    return (int)(want < most ? want : most);
 }
 
 extern "C" int ppo_token_logprobs(const ppo_token_logits* x, const void* tokens, int tokens_are_i64,
                                   const uint8_t* mask, float* logprobs, float* entropy, float* row_stats, void* stream) {
     const int e = check_logits(x, nullptr);
     if (e) return e;
-    const Logits L = logits_of(x, nullptr);
+    Logits L = logits_of(x, nullptr);
     if (L.n == 0) return 0;
     if (!tokens || !logprobs) return PPO_E_BADARG;
-    BY_TYPE_AND_THREADS(x->dtype, threads_of(L, x->dtype), T, NT, {
-        if (entropy) logprobs_kernel<T, NT, true><<<grid_of(L.n), NT, 0, (hipStream_t)stream>>>(
-            L, tokens, tokens_are_i64, mask, logprobs, nullptr, entropy, (RowStats*)row_stats);
-        else logprobs_kernel<T, NT, false><<<grid_of(L.n), NT, 0, (hipStream_t)stream>>>(
-            L, tokens, tokens_are_i64, mask, logprobs, nullptr, nullptr, (RowStats*)row_stats);
-    })
+    launch_logprobs(L, x->dtype, tokens, tokens_are_i64, mask, logprobs, nullptr, entropy, (RowStats*)row_stats,
+                    (hipStream_t)stream);
     return (int)hipGetLastError();
 }
 
-static int launch_backward(const Logits& L, int dtype, const void* tokens, int i64, const uint8_t* mask,
+static int launch_backward(Logits L, int dtype, const void* tokens, int i64, const uint8_t* mask,
                            const RowStats* stats, const Incoming& in, hipStream_t st) {
-    constexpr int NT = 256;
-    BY_TYPE(dtype, T, {
-        if (in.h) backward_kernel<T, NT, true><<<grid_of(L.n), NT, 0, st>>>(L, tokens, i64, mask, stats, in);
-        else backward_kernel<T, NT, false><<<grid_of(L.n), NT, 0, st>>>(L, tokens, i64, mask, stats, in);
-    })
+    BY_TYPE(dtype, T, BY_FLAG(by_wave(L, dtype), WAVE, BY_FLAG(in.h != nullptr, ENT, {
+        EACH_LAUNCH(L, WAVE, grid, (backward_kernel<T, WAVE, ENT><<<dim3(grid, WAVE ? 1 : backward_parts(L, dtype)), 256, 0, st>>>(
+            L, tokens, i64, mask, stats, in)))
+    })))
     return (int)hipGetLastError();
 }
 
@@ -916,7 +1150,7 @@ extern "C" int ppo_token_logprobs_backward(const ppo_token_logits* x, const void
                                            void* grad, void* stream) {
     const int e = check_logits(x, grad);
     if (e) return e;
-    const Logits L = logits_of(x, grad);
+    Logits L = logits_of(x, grad);
     if (L.n == 0) return 0;
     if (!tokens || !row_stats || !grad) return PPO_E_BADARG;
     const Incoming in = {grad_logprobs, grad_entropy, grad_factor, lp_seq_stride, lp_tok_stride, ent_seq_stride,
@@ -935,7 +1169,7 @@ extern "C" int ppo_policy_loss(const ppo_token_logits* x, const void* tokens, in
     const hipStream_t st = (hipStream_t)stream;
     const Workspace w = carve(workspace, x->n_seq, x->n_tok);
     if (!workspace || workspace_bytes < w.bytes) return PPO_E_WORKSPACE;
-    const Logits L = logits_of(x, grad);
+    Logits L = logits_of(x, grad);
     PolicyArgs p;
     e = weights_of(&p.w, mask, terms->reduction, terms->scale, x, w);
     if (e) return e;
@@ -958,14 +1192,23 @@ extern "C" int ppo_policy_loss(const ppo_token_logits* x, const void* tokens, in
         p.g_lp = seeds;
         p.g_h = seeds ? seeds + L.n : nullptr;
         p.part = w.part;
-        count_rows(mask, terms->reduction, x, w, st);
-        BY_TYPE_AND_THREADS(x->dtype, threads_of(L, x->dtype), T, NT, {
-            if (!grad) policy_kernel<T, NT, false, false><<<grid_of(L.n), NT, 0, st>>>(L, p);
-            else if (p.ent != 0.0f) policy_kernel<T, NT, true, true><<<grid_of(L.n), NT, 0, st>>>(L, p);
-            else policy_kernel<T, NT, true, false><<<grid_of(L.n), NT, 0, st>>>(L, p);
-        })
+        count_rows(p.w, x, w, st);
+        if (!grad) {
+            BY_TYPE(x->dtype, T, BY_FLAG(by_wave(L, x->dtype), WAVE, {
+                EACH_LAUNCH(L, WAVE, grid, (policy_forward_kernel<T, WAVE><<<grid, WAVE ? 256 : stream_threads(L), 0, st>>>(L, p)))
+            }))
+        } else {
+            BY_TYPE(x->dtype, T, BY_FLAG(p.ent != 0.0f, ENT, {
+                if (by_wave(L, x->dtype))
+                    EACH_LAUNCH(L, true, grid, (policy_kernel<T, 4, true, ENT><<<grid, 256, 0, st>>>(L, p)))
+                else if (held_in_8(L, x->dtype))
+                    EACH_LAUNCH(L, false, grid, (policy_kernel<T, 8, false, ENT><<<grid, held_threads(L, x->dtype, 8), 0, st>>>(L, p)))
+                else
+                    EACH_LAUNCH(L, false, grid, (policy_kernel<T, 16, false, ENT><<<grid, held_threads(L, x->dtype, 16), 0, st>>>(L, p)))
+            }))
+        }
     }
-    total_kernel<<<1, 1024, 0, st>>>(w.part, grid_of(L.n), loss);
+    launch_total(w, L.n, loss, st);
     return (int)hipGetLastError();
 }
 
@@ -979,18 +1222,17 @@ extern "C" int ppo_preference_loss(const ppo_token_logits* x, const void* tokens
     const hipStream_t st = (hipStream_t)stream;
     const Workspace w = carve(workspace, x->n_seq, x->n_tok);
     if (!workspace || workspace_bytes < w.bytes) return PPO_E_WORKSPACE;
-    const Logits L = logits_of(x, grad);
+    Logits L = logits_of(x, grad);
     if (L.n > 0 && !tokens) return PPO_E_BADARG;
     const int64_t pairs = x->n_seq / 2;
     RowStats* stats = row_stats ? (RowStats*)row_stats : w.stats;
     float* sd = seeds ? seeds : w.seeds;
     if (L.n > 0) {
-        BY_TYPE_AND_THREADS(x->dtype, threads_of(L, x->dtype), T, NT, (logprobs_kernel<T, NT, false><<<grid_of(L.n), NT, 0, st>>>(
-            L, tokens, tokens_are_i64, mask, nullptr, w.lp64, nullptr, stats)))
+        launch_logprobs(L, x->dtype, tokens, tokens_are_i64, mask, nullptr, w.lp64, nullptr, stats, st);
     }
-    pair_kernel<<<grid_of(pairs), 256, 0, st>>>(w.lp64, mask, ref_logprobs, pairs, x->n_tok, beta, label_smoothing, scale,
+    pair_kernel<<<(int)(pairs < LAUNCH_ROWS ? pairs : LAUNCH_ROWS), 256, 0, st>>>(w.lp64, mask, ref_logprobs, pairs, x->n_tok, beta, label_smoothing, scale,
                                                 rewards, sd, w.part);
-    total_kernel<<<1, 1024, 0, st>>>(w.part, (int)pairs, loss);
+    launch_total(w, pairs, loss, st);
     if (grad && L.n > 0) {
         const Incoming in = {sd, nullptr, nullptr, 1, 0, 0, 0};
         return launch_backward(L, x->dtype, tokens, tokens_are_i64, mask, stats, in, st);
@@ -1027,18 +1269,23 @@ extern "C" int ppo_distillation_loss(const ppo_token_logits* x, const void* teac
     if (!workspace || workspace_bytes < w.bytes) return PPO_E_WORKSPACE;
     e = weights_of(&p.w, mask, reduction, scale, x, w);
     if (e) return e;
-    const Logits L = logits_of(x, grad);
+    Logits L = logits_of(x, grad);
     p.losses = token_losses;
     p.stats = (RowStats*)row_stats;
     p.part = w.part;
     if (L.n > 0) {
-        count_rows(mask, reduction, x, w, st);
-        BY_TYPE_AND_THREADS(x->dtype, threads_of(L, x->dtype), T, NT, {
-            if (grad) distill_kernel<T, NT, true><<<grid_of(L.n), NT, 0, st>>>(L, p);
-            else distill_kernel<T, NT, false><<<grid_of(L.n), NT, 0, st>>>(L, p);
+        count_rows(p.w, x, w, st);
+        const size_t lds = teacher_lds(top);
+        BY_TYPE(x->dtype, T, {
+            if (!grad)
+                EACH_LAUNCH(L, false, grid, (distill_forward_kernel<T><<<grid, stream_threads(L), lds, st>>>(L, p)))
+            else if (held_in_8(L, x->dtype))
+                EACH_LAUNCH(L, false, grid, (distill_kernel<T, 8><<<grid, held_threads(L, x->dtype, 8), lds, st>>>(L, p)))
+            else
+                EACH_LAUNCH(L, false, grid, (distill_kernel<T, 16><<<grid, held_threads(L, x->dtype, 16), lds, st>>>(L, p)))
         })
     }
-    total_kernel<<<1, 1024, 0, st>>>(w.part, grid_of(L.n), loss);
+    launch_total(w, L.n, loss, st);
     return (int)hipGetLastError();
 }
 
@@ -1049,13 +1296,12 @@ extern "C" int ppo_distillation_backward(const ppo_token_logits* x, const void* 
     TeacherArgs p;
     if (!e) e = teacher_of(&p, x, teacher_tokens, tokens_are_i64, teacher_logits, teacher_dtype, top);
     if (e) return e;
-    const Logits L = logits_of(x, grad);
+    Logits L = logits_of(x, grad);
     if (L.n == 0) return 0;
     if (!row_stats || !grad) return PPO_E_BADARG;
     p.w.mask = mask;
     p.stats = (RowStats*)row_stats;
     p.factor = grad_factor;
-    constexpr int NT = 256;
-    BY_TYPE(x->dtype, T, (distill_backward_kernel<T, NT><<<grid_of(L.n), NT, 0, (hipStream_t)stream>>>(L, p)))
+    BY_TYPE(x->dtype, T, EACH_LAUNCH(L, false, grid, (distill_backward_kernel<T><<<grid, 256, teacher_lds(top), (hipStream_t)stream>>>(L, p))))
     return (int)hipGetLastError();
 }

@@ -75,7 +75,7 @@ def logits_struct(**more):
 
 BAD_LOGITS = [(dict(dtype=3), -1), (dict(vocab=0), -1), (dict(n_seq=-1), -1), (dict(inv_temperature=0.0), -1),
               (dict(inv_temperature=float("nan")), -1), (dict(inv_temperature=float("inf")), -1), (dict(data=None), -1),
-              (dict(data=(1 << 20) + 2), -1), (dict(vocab=(1 << 30) + 1), -3), (dict(n_seq=1 << 20, n_tok=1 << 20), -3)]
+              (dict(data=(1 << 20) + 2), -1), (dict(vocab=(1 << 26) + 1), -3), (dict(n_seq=1 << 20, n_tok=1 << 20), -3)]
 BAD_GRADS = [(dict(grad_tok_stride=9), -1), (dict(grad_seq_stride=39), -1), (dict(grad_tok_stride=0), -1)]
 
 
