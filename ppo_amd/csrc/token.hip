@@ -218,18 +218,28 @@ template <typename T> struct Span {
     }
 };
 
-// vector j of the body; the gradient's may lie across a boundary
-template <typename T> __device__ __forceinline__ u32x4 load_vec(const T* body, int j) {
-    return *(const u32x4*)((const char*)body + 16u * (uint32_t)j);
+// Vector j of the body.  KEEP: it will be read again, and a non-temporal load would let the caches drop it.
+template <bool KEEP, typename T> __device__ __forceinline__ u32x4 load_vec(const T* body, int j) {
+    const u32x4* at = (const u32x4*)((const char*)body + 16u * (uint32_t)j);
+    return KEEP ? *at : __builtin_nontemporal_load(at);
 }
-template <typename T> __device__ __forceinline__ void store_vec(T* body, int j, u32x4 o) {
-    __builtin_memcpy((char*)body + 16u * (uint32_t)j, &o, 16);
+// Of the gradient, whose vectors may lie across a boundary.  past: not through the caches.
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+template <typename T> __device__ __forceinline__ void store_vec(T* body, int j, u32x4 o, bool past) {
+    u32x4_any* at = (u32x4_any*)((char*)body + 16u * (uint32_t)j);
+    if (past) {
+        asm volatile("");     // or the compiler makes one ordinary store of the two
+        __builtin_nontemporal_store(o, at);
+        asm volatile("");
+    } else {
+        *at = o;
+    }
 }
 
 // (m, S, E) of a row that is not kept, joined over the wave.  STREAM vectors of a thread are on their way while the
 // STREAM before are added.
 #define STREAM 4
-template <typename T, bool ENT, bool NEAR>
+template <typename T, bool ENT, bool NEAR, bool KEEP>
 __device__ __forceinline__ Acc stream_stats(const T* x, int V, float c2, const Part p, float counted) {
     constexpr int N = VEC<T>;
     const Span<T> s(x, V);
@@ -244,7 +254,7 @@ __device__ __forceinline__ Acc stream_stats(const T* x, int V, float c2, const P
         const T* from = body;
         auto fetch = [&]() {          // a step of which every thread has its part
 #pragma unroll
-            for (int k = 0; k < STREAM; ++k) next[k] = load_vec(from + (int64_t)k * p.nt * N, p.tid);
+            for (int k = 0; k < STREAM; ++k) next[k] = load_vec<KEEP>(from + (int64_t)k * p.nt * N, p.tid);
         };
         if (steps > 0) fetch();
         for (int i = 1; i < steps; ++i) {
@@ -261,7 +271,7 @@ __device__ __forceinline__ Acc stream_stats(const T* x, int V, float c2, const P
         }
         // the last step, which may be empty: threads without a part read the last vector of the row
 #pragma unroll
-        for (int k = 0; k < STREAM; ++k) next[k] = load_vec(body, min(steps * step + k * p.nt + p.tid, s.nvec - 1));
+        for (int k = 0; k < STREAM; ++k) next[k] = load_vec<KEEP>(body, min(steps * step + k * p.nt + p.tid, s.nvec - 1));
         __builtin_amdgcn_sched_barrier(0);
         if (steps > 0) acc_vecs<T, STREAM, ENT, NEAR>(a, v, c2);
 #pragma unroll
@@ -277,9 +287,9 @@ __device__ __forceinline__ Acc stream_stats(const T* x, int V, float c2, const P
 }
 
 // The same joined over the workgroup in its first wave: true there, and the other waves are done.
-template <typename T, bool WAVE, bool ENT>
+template <typename T, bool WAVE, bool ENT, bool KEEP>
 __device__ __forceinline__ bool stream_row(const T* x, int V, float c2, float counted, Acc* lds, Acc& a) {
-    a = stream_stats<T, ENT, true>(x, V, c2, part_of<WAVE>(), counted);
+    a = stream_stats<T, ENT, true, KEEP>(x, V, c2, part_of<WAVE>(), counted);
     if (!WAVE) {
         if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
         __syncthreads();
@@ -288,7 +298,7 @@ __device__ __forceinline__ bool stream_row(const T* x, int V, float c2, float co
     }
     const float n = a.n;
     if (is_near(a.m, c2)) a = near_done(a, c2);
-    else a = stream_stats<T, ENT, false>(x, V, c2, part_of<true>(), 0.0f);
+    else a = stream_stats<T, ENT, false, true>(x, V, c2, part_of<true>(), 0.0f);
     a.n = n;
     return true;
 }
@@ -308,7 +318,7 @@ __device__ __forceinline__ void row_load(Row<T, CH>& row, const T* x, const Span
     row.edge = e >= 0 ? wide(x[e]) : -__builtin_inff();
     if (s.nvec > 0) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) row.v[i] = load_vec(x + s.head, min(i * p.nt + p.tid, s.nvec - 1));
+        for (int i = 0; i < CH; ++i) row.v[i] = load_vec<false>(x + s.head, min(i * p.nt + p.tid, s.nvec - 1));
     }
 }
 
@@ -330,7 +340,7 @@ __device__ __forceinline__ Acc row_stats(Row<T, CH>& row, const T* x, const Span
     }
     if (CH == 16)
         for (int j = CH * p.nt + p.tid; j < s.nvec; j += p.nt) {
-            const u32x4 v = load_vec(x + s.head, j);
+            const u32x4 v = load_vec<true>(x + s.head, j);
             acc_vecs<T, 1, ENT>(a, &v, c2);
         }
     acc_rebase<ENT>(a, fmaxf(a.m, row.edge), c2);
@@ -379,7 +389,7 @@ __device__ __forceinline__ void edge_grad(const RowGrad& g, float x, T* out, int
 // The gradient of a held row.  The vectors that are read again may lie where their gradient goes.
 template <typename T, int CH, bool ENT>
 __device__ __forceinline__ void row_grad(const Row<T, CH>& row, const T* x, T* out, const Span<T>& s, const Part& p,
-                                         float c2, const RowGrad& g) {
+                                         float c2, const RowGrad& g, bool past) {
     constexpr int N = VEC<T>;
     const int mine = s.nvec - p.first;
     const int tok = g.tok >= 0 ? g.tok - s.head : -1;
@@ -388,34 +398,34 @@ __device__ __forceinline__ void row_grad(const Row<T, CH>& row, const T* x, T* o
         if (i * p.nt < mine) {
             const int j = i * p.nt + p.tid;
             const u32x4 o = grad_vec<T, ENT>(g, row.v[i], tok - j * N, c2);
-            if (j < s.nvec) store_vec(out + s.head, j, o);
+            if (j < s.nvec) store_vec(out + s.head, j, o, past);
         }
     }
     if (CH == 16)
         for (int j = CH * p.nt + p.tid; j < s.nvec; j += p.nt)
-            store_vec(out + s.head, j, grad_vec<T, ENT>(g, load_vec(x + s.head, j), tok - j * N, c2));
+            store_vec(out + s.head, j, grad_vec<T, ENT>(g, load_vec<false>(x + s.head, j), tok - j * N, c2), past);
     edge_grad<T, ENT>(g, row.edge, out, s.edge(p.tid), c2);
 }
 
 // The gradient of a row whose statistics are known, vectors j0 up to j1; x may be out.
 template <typename T, bool ENT>
 __device__ __forceinline__ void row_map(const T* x, T* out, int V, const Part& p, int seg, int segs, float c2,
-                                        const RowGrad& g) {
+                                        const RowGrad& g, bool past) {
     constexpr int N = VEC<T>;
     const Span<T> s(x, V);
     const int per = (s.nvec + segs - 1) / segs, end = min(s.nvec, (seg + 1) * per);
     const int tok = g.tok >= 0 ? g.tok - s.head : -1;
     for (int j = seg * per + p.tid; j < end; j += p.nt)
-        store_vec(out + s.head, j, grad_vec<T, ENT>(g, load_vec(x + s.head, j), tok - j * N, c2));
+        store_vec(out + s.head, j, grad_vec<T, ENT>(g, load_vec<false>(x + s.head, j), tok - j * N, c2), past);
     const int e = seg == 0 ? s.edge(p.tid) : -1;
     edge_grad<T, ENT>(g, e >= 0 ? wide(x[e]) : 0.0f, out, e, c2);
 }
 
-template <typename T> __device__ __forceinline__ void row_fill(T* out, int V, const Part& p, int seg = 0, int segs = 1) {
+template <typename T> __device__ __forceinline__ void row_fill(T* out, int V, const Part& p, int seg, int segs, bool past) {
     const Span<T> s(out, V);
     const int per = (s.nvec + segs - 1) / segs, end = min(s.nvec, (seg + 1) * per);
     const u32x4 zero = 0;
-    for (int j = seg * per + p.tid; j < end; j += p.nt) store_vec(out + s.head, j, zero);
+    for (int j = seg * per + p.tid; j < end; j += p.nt) store_vec(out + s.head, j, zero, past);
     const int e = seg == 0 ? s.edge(p.tid) : -1;
     if (e >= 0) out[e] = (T)0.0f;
 }
@@ -429,9 +439,10 @@ struct Logits {
     int64_t r0;               // first row of this launch
     int V;
     float c, c2;              // 1/temperature; the same times log2(e)
+    bool past;                // the gradient is stored past the caches
 };
 
-template <bool WAVE> __device__ __forceinline__ int64_t row_of(const Logits& L) {
+template <bool WAVE> __device__ __forceinline__ int64_t row_of(const Logits& L) {   // (one workgroup may have 16 waves)
     return L.r0 + (WAVE ? (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : (int64_t)blockIdx.x);
 }
 
@@ -577,7 +588,7 @@ __global__ __launch_bounds__(1024) void total_kernel(const double* __restrict__ 
 }
 
 // ------------------------------------------------------------------------------------------ log-probabilities
-template <typename T, bool WAVE, bool ENT>
+template <typename T, bool WAVE, bool ENT, bool KEEP>
 __global__ __launch_bounds__(1024, 4) void logprobs_kernel(Logits L, const void* tokens, int i64, const uint8_t* mask,
                                                            float* logprobs, double* logprobs64, float* entropy,
                                                            RowStats* stats) {
@@ -590,7 +601,7 @@ __global__ __launch_bounds__(1024, 4) void logprobs_kernel(Logits L, const void*
         const T* x = row_in<T>(L, place_of(L, r));
         const float xt = token_logit(x, int_at(tokens, i64, r), L.V);
         Acc a;
-        if (!stream_row<T, WAVE, ENT>(x, L.V, L.c2, 0.0f, lds, a)) return;
+        if (!stream_row<T, WAVE, ENT, KEEP>(x, L.V, L.c2, 0.0f, lds, a)) return;
         const double ln_s = ln_of(a.s);
         lp = logp_of(xt, L.c, a, ln_s);
         st.m = a.m;
@@ -623,16 +634,17 @@ struct Incoming {             // dL/dlogp and dL/dH of each row, and a factor on
     int64_t lp_s, lp_t, h_s, h_t;
 };
 
+// Rows in the reverse of the forward pass's order: what it read last is still in the 256 MB cache in front of the HBM.
 template <typename T, bool WAVE, bool ENT>
 __global__ __launch_bounds__(256) void backward_kernel(Logits L, const void* tokens, int i64, const uint8_t* mask,
                                                        const RowStats* __restrict__ stats, Incoming in) {
-    const int64_t r = row_of<WAVE>(L);
-    if (WAVE && r >= L.n) return;
+    const int64_t r = L.n - 1 - row_of<WAVE>(L);
+    if (WAVE && r < 0) return;
     const Part p = part_of<WAVE>();
     const Place at = place_of(L, r);
     T* out = row_out<T>(L, at);
     if (mask && !mask[r]) {
-        row_fill(out, L.V, p, blockIdx.y, gridDim.y);
+        row_fill(out, L.V, p, blockIdx.y, gridDim.y, L.past);
         return;
     }
     const float f = in.factor ? *in.factor : 1.0f;
@@ -640,7 +652,7 @@ __global__ __launch_bounds__(256) void backward_kernel(Logits L, const void* tok
     const float g_lp = in.lp ? f * in.lp[at.b * in.lp_s + at.t * in.lp_t] : 0.0f;
     const float g_h = ENT ? f * in.h[at.b * in.h_s + at.t * in.h_t] : 0.0f;
     const RowGrad g = grad_seed(st.m, st.s, st.h, g_lp, g_h, int_at(tokens, i64, r), L.V, L.c);
-    row_map<T, ENT>(row_in<T>(L, at), out, L.V, p, blockIdx.y, gridDim.y, L.c2, g);
+    row_map<T, ENT>(row_in<T>(L, at), out, L.V, p, blockIdx.y, gridDim.y, L.c2, g, L.past);
 }
 
 // ------------------------------------------------------------------------------------------ clipped policy loss
@@ -655,6 +667,7 @@ struct PolicyArgs {
     RowStats* stats;          // with seeds: the differentiable form
     float *g_lp, *g_h;
     double* part;             // weighted loss of each row
+    float* solo;              // the loss, where one workgroup has all rows
 };
 
 struct PolicyRow {
@@ -701,74 +714,97 @@ __device__ __forceinline__ PolicyIn policy_in(const Logits& L, const PolicyArgs&
     return i;
 }
 
+// The weighted loss of row r: left to total_kernel, or, where this workgroup has all rows, summed over its waves in their
+// order (every wave comes here then, with 0 where it had no row).
+template <bool WAVE> __device__ __forceinline__ void row_loss(const PolicyArgs& p, int64_t r, int64_t n, double loss) {
+    if (!p.solo) {
+        if (part_of<WAVE>().tid == 0 && r < n) p.part[r] = loss;
+        return;
+    }
+    __shared__ double sums[16];
+    if (WAVE) {
+        if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = loss;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            loss = 0.0;
+            for (int w = 0; w < (int)blockDim.x / 64; ++w) loss += sums[w];
+        }
+    }
+    if (threadIdx.x == 0) *p.solo = (float)loss;
+}
+
 // Forward only; leaves what the backward pass needs.
 template <typename T, bool WAVE>
 __global__ __launch_bounds__(1024, 4) void policy_forward_kernel(Logits L, PolicyArgs p) {
     __shared__ Acc lds[16];
     const int64_t r = row_of<WAVE>(L);
-    if (WAVE && r >= L.n) return;
-    RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
-    double lp = 0.0;
     PolicyRow o = {0.0, 0.0f, 0.0f};
-    if (!p.w.mask || p.w.mask[r]) {
-        const Place at = place_of(L, r);
-        const T* x = row_in<T>(L, at);
-        const PolicyIn in = policy_in(L, p, x, r, at);
-        Acc a;
-        if (!stream_row<T, WAVE, true>(x, L.V, L.c2, count_mask(p.w, L.n, part_of<WAVE>()), lds, a)) return;
-        const double ln_s = ln_of(a.s);
-        lp = logp_of(in.xt, L.c, a, ln_s);
-        st.m = a.m;
-        st.s = a.s;
-        st.h = entropy_of(a, ln_s);
-        o = policy_row(p, lp, st.h, in.old_lp, in.adv, in.ref, row_weight(p.w, at, L.n_tok, a.n));
-    }
-    if (part_of<WAVE>().tid == 0) {
-        p.logprobs[r] = (float)lp;
-        if (p.entropy) p.entropy[r] = st.h;
-        if (p.stats) {
-            p.stats[r] = st;
-            p.g_lp[r] = o.g_lp;
-            p.g_h[r] = o.g_h;
+    if (!WAVE || r < L.n) {
+        RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
+        double lp = 0.0;
+        if (!p.w.mask || p.w.mask[r]) {
+            const Place at = place_of(L, r);
+            const T* x = row_in<T>(L, at);
+            const PolicyIn in = policy_in(L, p, x, r, at);
+            Acc a;
+            if (!stream_row<T, WAVE, true, true>(x, L.V, L.c2, count_mask(p.w, L.n, part_of<WAVE>()), lds, a)) return;
+            const double ln_s = ln_of(a.s);
+            lp = logp_of(in.xt, L.c, a, ln_s);
+            st.m = a.m;
+            st.s = a.s;
+            st.h = entropy_of(a, ln_s);
+            o = policy_row(p, lp, st.h, in.old_lp, in.adv, in.ref, row_weight(p.w, at, L.n_tok, a.n));
         }
-        p.part[r] = o.loss;
+        if (part_of<WAVE>().tid == 0) {
+            p.logprobs[r] = (float)lp;
+            if (p.entropy) p.entropy[r] = st.h;
+            if (p.stats) {
+                p.stats[r] = st;
+                p.g_lp[r] = o.g_lp;
+                p.g_h[r] = o.g_h;
+            }
+        }
     }
+    row_loss<WAVE>(p, r, L.n, o.loss);
 }
 
 // Loss and gradient: the row stays on the chip between its statistics and its gradient.
 template <typename T, int CH, bool WAVE, bool ENT_GRAD>
-__global__ __launch_bounds__(WAVE ? 256 : 1024, 4) void policy_kernel(Logits L, PolicyArgs p) {
+__global__ __launch_bounds__(1024, 4) void policy_kernel(Logits L, PolicyArgs p) {
     __shared__ Acc lds[16];
-    const int64_t r = row_of<WAVE>(L);
-    if (WAVE && r >= L.n) return;
     const Part q = part_of<WAVE>();
-    const Place at = place_of(L, r);
-    T* out = row_out<T>(L, at);
-    double lp = 0.0, loss = 0.0;
-    float h = 0.0f;
-    if (!p.w.mask || p.w.mask[r]) {
-        const T* x = row_in<T>(L, at);
-        const Span<T> s(x, L.V);
-        Row<T, CH> row;
-        const PolicyIn in = policy_in(L, p, x, r, at);
-        row_load(row, x, s, q);
-        const float counted = count_mask(p.w, L.n, q);
-        asm volatile("" :: "v"(in.xt));   // read before the barrier in row_stats: the gradient may overwrite it
-        const Acc a = row_stats<T, CH, WAVE, true>(row, x, s, q, L.c2, counted, lds);
-        const double ln_s = ln_of(a.s);
-        lp = logp_of(in.xt, L.c, a, ln_s);
-        h = entropy_of(a, ln_s);
-        const PolicyRow o = policy_row(p, lp, h, in.old_lp, in.adv, in.ref, row_weight(p.w, at, L.n_tok, a.n));
-        loss = o.loss;
-        row_grad<T, CH, ENT_GRAD>(row, x, out, s, q, L.c2, grad_seed(a.m, a.s, h, o.g_lp, o.g_h, in.tok, L.V, L.c));
-    } else {
-        row_fill(out, L.V, q);
+    const int64_t r = row_of<WAVE>(L);
+    double loss = 0.0;
+    if (!WAVE || r < L.n) {
+        const Place at = place_of(L, r);
+        T* out = row_out<T>(L, at);
+        double lp = 0.0;
+        float h = 0.0f;
+        if (!p.w.mask || p.w.mask[r]) {
+            const T* x = row_in<T>(L, at);
+            const Span<T> s(x, L.V);
+            Row<T, CH> row;
+            const PolicyIn in = policy_in(L, p, x, r, at);
+            row_load(row, x, s, q);
+            const float counted = count_mask(p.w, L.n, q);
+            asm volatile("" :: "v"(in.xt));   // read before the barrier in row_stats: the gradient may overwrite it
+            const Acc a = row_stats<T, CH, WAVE, true>(row, x, s, q, L.c2, counted, lds);
+            const double ln_s = ln_of(a.s);
+            lp = logp_of(in.xt, L.c, a, ln_s);
+            h = entropy_of(a, ln_s);
+            const PolicyRow o = policy_row(p, lp, h, in.old_lp, in.adv, in.ref, row_weight(p.w, at, L.n_tok, a.n));
+            loss = o.loss;
+            row_grad<T, CH, ENT_GRAD>(row, x, out, s, q, L.c2, grad_seed(a.m, a.s, h, o.g_lp, o.g_h, in.tok, L.V, L.c),
+                                      L.past);
+        } else {
+            row_fill(out, L.V, q, 0, 1, L.past);
+        }
+        if (q.tid == 0) {
+            p.logprobs[r] = (float)lp;
+            if (p.entropy) p.entropy[r] = h;
+        }
     }
-    if (q.tid == 0) {
-        p.logprobs[r] = (float)lp;
-        if (p.entropy) p.entropy[r] = h;
-        p.part[r] = loss;
-    }
+    row_loss<WAVE>(p, r, L.n, loss);
 }
 
 // ------------------------------------------------------------------------------------------ preference loss
@@ -776,7 +812,7 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024, 4) void policy_kernel(Logits L, 
 __global__ __launch_bounds__(256) void pair_kernel(const double* __restrict__ lp, const uint8_t* __restrict__ mask,
                                                    const float* __restrict__ ref, int64_t n_pairs, int64_t n_tok,
                                                    double beta, double smooth, double scale, float* rewards,
-                                                   float* seeds, double* part) {
+                                                   float* seeds, double* part, float* solo) {
     __shared__ double lds[4];
     for (int64_t q = blockIdx.x; q < n_pairs; q += gridDim.x) {
         double s[2];
@@ -796,7 +832,9 @@ __global__ __launch_bounds__(256) void pair_kernel(const double* __restrict__ lp
             const double z = s[0] - s[1], t = exp(-fabs(z)), l = log1p(t);   // ln(1 + e^-|z|)
             const double neg = (z > 0.0 ? 0.0 : -z) + l, pos = (z > 0.0 ? z : 0.0) + l;   // -ln sig(z), -ln sig(-z); NaN stays in l
             const double sig = z > 0.0 ? 1.0 / (1.0 + t) : t / (1.0 + t);
-            part[q] = scale * ((1.0 - smooth) * neg + (smooth != 0.0 ? smooth * pos : 0.0)) / (double)n_pairs;   // pos may be inf
+            const double loss = scale * ((1.0 - smooth) * neg + (smooth != 0.0 ? smooth * pos : 0.0)) / (double)n_pairs;   // pos may be inf
+            if (solo) *solo = (float)loss;     // the only pair
+            else part[q] = loss;
             const float g = (float)(scale * beta * (sig - (1.0 - smooth)) / (double)n_pairs);
             rewards[q] = (float)s[0];
             rewards[q + n_pairs] = (float)s[1];
@@ -815,6 +853,7 @@ struct TeacherArgs {
     RowStats* stats;
     const float* factor;
     double* part;
+    float* solo;              // the loss, where there is one row
 };
 
 // One row's entries, K of each array in LDS.  The first wave makes them while the others wait for their logits.
@@ -909,7 +948,7 @@ __global__ __launch_bounds__(1024, 4) void distill_forward_kernel(Logits L, Teac
         float ent = 0.0f;
         if (threadIdx.x < 64) ent = teacher_load(p, L, r, x, teach);
         Acc a;
-        if (!stream_row<T, false, false>(x, L.V, L.c2, count_mask(p.w, L.n, part_of<false>()), lds, a)) return;
+        if (!stream_row<T, false, false, true>(x, L.V, L.c2, count_mask(p.w, L.n, part_of<false>()), lds, a)) return;
         loss = teacher_loss(p, teach, ent, a, L.c) / (L.c * L.c);
         st.m = a.m;
         st.s = a.s;
@@ -918,7 +957,8 @@ __global__ __launch_bounds__(1024, 4) void distill_forward_kernel(Logits L, Teac
     if (threadIdx.x == 0) {
         if (p.losses) p.losses[r] = loss;
         if (p.stats) p.stats[r] = st;
-        p.part[r] = (double)st.w * (double)loss;
+        if (p.solo) *p.solo = (float)((double)st.w * (double)loss);
+        else p.part[r] = (double)st.w * (double)loss;
     }
 }
 
@@ -942,27 +982,28 @@ __global__ __launch_bounds__(1024, 4) void distill_kernel(Logits L, TeacherArgs 
         const Acc a = row_stats<T, CH, false, false>(row, x, s, q, L.c2, count_mask(p.w, L.n, q), lds);
         w = row_weight(p.w, at, L.n_tok, a.n);
         const RowGrad g = teacher_seed(teach, a.m, a.s, w / L.c);
-        row_grad<T, CH, false>(row, x, out, s, q, L.c2, g);
+        row_grad<T, CH, false>(row, x, out, s, q, L.c2, g, L.past);
         teacher_places(p, teach, out, L, g, w / L.c);
         if (q.first == 0) loss = teacher_loss(p, teach, ent, a, L.c) / (L.c * L.c);
     } else {
-        row_fill(out, L.V, q);
+        row_fill(out, L.V, q, 0, 1, L.past);
     }
     if (threadIdx.x == 0) {
         if (p.losses) p.losses[r] = loss;
-        p.part[r] = (double)w * (double)loss;
+        if (p.solo) *p.solo = (float)((double)w * (double)loss);
+        else p.part[r] = (double)w * (double)loss;
     }
 }
 
 template <typename T> __global__ __launch_bounds__(256) void distill_backward_kernel(Logits L, TeacherArgs p) {
     extern __shared__ int entries[];
     const Teacher teach(entries, p.K);
-    const int64_t r = row_of<false>(L);
+    const int64_t r = L.n - 1 - row_of<false>(L);   // as in backward_kernel
     const Part q = part_of<false>();
     const Place at = place_of(L, r);
     T* out = row_out<T>(L, at);
     if (p.w.mask && !p.w.mask[r]) {
-        row_fill(out, L.V, q);
+        row_fill(out, L.V, q, 0, 1, L.past);
         return;
     }
     const T* x = row_in<T>(L, at);
@@ -971,7 +1012,7 @@ template <typename T> __global__ __launch_bounds__(256) void distill_backward_ke
     const RowStats st = p.stats[r];
     const float g = (p.factor ? *p.factor : 1.0f) * st.w / L.c;
     const RowGrad rg = teacher_seed(teach, st.m, st.s, g);
-    row_map<T, false>(x, out, L.V, q, 0, 1, L.c2, rg);
+    row_map<T, false>(x, out, L.V, q, 0, 1, L.c2, rg, L.past);
     teacher_places(p, teach, out, L, rg, g);
 }
 
@@ -1040,6 +1081,9 @@ static Logits logits_of(const ppo_token_logits* x, void* grad) {
     L.V = (int)x->vocab;
     L.c = x->inv_temperature;
     L.c2 = x->inv_temperature * LOG2E_F;
+    // A gradient that the 256 MB cache cannot hold is stored past it: 32768 bf16 logits a row, loss and gradient and a
+    // copy of the gradient after it take 200 us against 208 at 256 MB, but 99 against 81 at 128 MB.
+    L.past = L.n * L.V * (x->dtype == PPO_F32 ? 4 : 2) > (int64_t)192 << 20;
     return L;
 }
 
@@ -1055,6 +1099,8 @@ static int64_t row_bytes(const Logits& L, int dtype) { return (int64_t)L.V * (dt
 
 // A wave takes a row of up to 4 KB by itself: its 64 lanes hold that in four vectors each.
 static bool by_wave(const Logits& L, int dtype) { return row_bytes(L, dtype) <= 4096; }
+
+#define SOLO_ROWS 16
 
 // A launch takes LAUNCH_ROWS rows at most: a grid of 2^32 threads and more is refused.  Runs its arguments for each
 // launch with the rows' first in L.r0 and `grid` workgroups of a row, or of four (WAVE).
@@ -1110,10 +1156,10 @@ static int weights_of(Weights* o, const uint8_t* mask, int reduction, float scal
 
 static void launch_logprobs(Logits L, int dtype, const void* tokens, int i64, const uint8_t* mask, float* logprobs,
                             double* logprobs64, float* entropy, RowStats* stats, hipStream_t st) {
-    BY_TYPE(dtype, T, BY_FLAG(by_wave(L, dtype), WAVE, BY_FLAG(entropy != nullptr, ENT, {
-        EACH_LAUNCH(L, WAVE, grid, (logprobs_kernel<T, WAVE, ENT><<<grid, WAVE ? 256 : stream_threads(L), 0, st>>>(
+    BY_TYPE(dtype, T, BY_FLAG(by_wave(L, dtype), WAVE, BY_FLAG(entropy != nullptr, ENT, BY_FLAG(stats != nullptr, KEEP, {
+        EACH_LAUNCH(L, WAVE, grid, (logprobs_kernel<T, WAVE, ENT, KEEP><<<grid, WAVE ? 256 : stream_threads(L), 0, st>>>(
             L, tokens, i64, mask, logprobs, logprobs64, entropy, stats)))
-    })))
+    }))))
 }
 
 // Parts of a row that the backward pass gives to a workgroup each, so that few rows fill the chip too: at least 16 KB.
@@ -1171,6 +1217,7 @@ extern "C" int ppo_policy_loss(const ppo_token_logits* x, const void* tokens, in
     if (!workspace || workspace_bytes < w.bytes) return PPO_E_WORKSPACE;
     Logits L = logits_of(x, grad);
     PolicyArgs p;
+    bool solo = false;
     e = weights_of(&p.w, mask, terms->reduction, terms->scale, x, w);
     if (e) return e;
     if (L.n > 0) {
@@ -1192,15 +1239,18 @@ extern "C" int ppo_policy_loss(const ppo_token_logits* x, const void* tokens, in
         p.g_lp = seeds;
         p.g_h = seeds ? seeds + L.n : nullptr;
         p.part = w.part;
+        // One workgroup, of a wave for each row, where that takes them all: the loss then needs no second launch.
+        solo = L.n == 1 || (by_wave(L, x->dtype) && L.n <= SOLO_ROWS);
+        p.solo = solo ? loss : nullptr;
         count_rows(p.w, x, w, st);
         if (!grad) {
             BY_TYPE(x->dtype, T, BY_FLAG(by_wave(L, x->dtype), WAVE, {
-                EACH_LAUNCH(L, WAVE, grid, (policy_forward_kernel<T, WAVE><<<grid, WAVE ? 256 : stream_threads(L), 0, st>>>(L, p)))
+                EACH_LAUNCH(L, WAVE, grid, (policy_forward_kernel<T, WAVE><<<solo ? 1 : grid, WAVE ? solo ? 64 * (int)L.n : 256 : stream_threads(L), 0, st>>>(L, p)))
             }))
         } else {
             BY_TYPE(x->dtype, T, BY_FLAG(p.ent != 0.0f, ENT, {
                 if (by_wave(L, x->dtype))
-                    EACH_LAUNCH(L, true, grid, (policy_kernel<T, 4, true, ENT><<<grid, 256, 0, st>>>(L, p)))
+                    EACH_LAUNCH(L, true, grid, (policy_kernel<T, 4, true, ENT><<<solo ? 1 : grid, solo ? 64 * (int)L.n : 256, 0, st>>>(L, p)))
                 else if (held_in_8(L, x->dtype))
                     EACH_LAUNCH(L, false, grid, (policy_kernel<T, 8, false, ENT><<<grid, held_threads(L, x->dtype, 8), 0, st>>>(L, p)))
                 else
@@ -1208,7 +1258,7 @@ extern "C" int ppo_policy_loss(const ppo_token_logits* x, const void* tokens, in
             }))
         }
     }
-    launch_total(w, L.n, loss, st);
+    if (!solo) launch_total(w, L.n, loss, st);
     return (int)hipGetLastError();
 }
 
@@ -1231,8 +1281,8 @@ extern "C" int ppo_preference_loss(const ppo_token_logits* x, const void* tokens
         launch_logprobs(L, x->dtype, tokens, tokens_are_i64, mask, nullptr, w.lp64, nullptr, stats, st);
     }
     pair_kernel<<<(int)(pairs < LAUNCH_ROWS ? pairs : LAUNCH_ROWS), 256, 0, st>>>(w.lp64, mask, ref_logprobs, pairs, x->n_tok, beta, label_smoothing, scale,
-                                                rewards, sd, w.part);
-    launch_total(w, pairs, loss, st);
+                                                rewards, sd, w.part, pairs == 1 ? loss : nullptr);
+    if (pairs > 1) launch_total(w, pairs, loss, st);
     if (grad && L.n > 0) {
         const Incoming in = {sd, nullptr, nullptr, 1, 0, 0, 0};
         return launch_backward(L, x->dtype, tokens, tokens_are_i64, mask, stats, in, st);
@@ -1273,6 +1323,7 @@ extern "C" int ppo_distillation_loss(const ppo_token_logits* x, const void* teac
     p.losses = token_losses;
     p.stats = (RowStats*)row_stats;
     p.part = w.part;
+    p.solo = L.n == 1 ? loss : nullptr;
     if (L.n > 0) {
         count_rows(p.w, x, w, st);
         const size_t lds = teacher_lds(top);
@@ -1285,7 +1336,7 @@ extern "C" int ppo_distillation_loss(const ppo_token_logits* x, const void* teac
                 EACH_LAUNCH(L, false, grid, (distill_kernel<T, 16><<<grid, held_threads(L, x->dtype, 16), lds, st>>>(L, p)))
         })
     }
-    launch_total(w, L.n, loss, st);
+    if (L.n != 1) launch_total(w, L.n, loss, st);
     return (int)hipGetLastError();
 }
 

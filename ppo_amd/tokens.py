@@ -39,6 +39,7 @@ MAX_TEACHER_TOP = 512
 
 
 # ------------------------------------------------------------------------------------------ arguments
+# The checks are written for their cost: a call on a few rows is host time and little else.
 def _check_logits(logits):
     if not isinstance(logits, torch.Tensor) or logits.dim() not in (2, 3):
         raise ValueError("logits must be a tensor [sequences, tokens, vocabulary] or [tokens, vocabulary]")
@@ -46,44 +47,40 @@ def _check_logits(logits):
         raise ValueError(f"logits of type {logits.dtype}: float32, bfloat16 and float16 are supported")
     if logits.shape[-1] < 1:
         raise ValueError("logits over an empty vocabulary")
-    if logits.shape[-1] > 1 and logits.stride(-1) != 1:
+    if logits.stride(-1) != 1 and logits.shape[-1] > 1:
         raise ValueError("the vocabulary must be the contiguous dimension of the logits")
+    return logits.shape[:-1]
 
 
-def _same_device(logits, t, name):
-    if not isinstance(t, torch.Tensor) or t.device != logits.device:
+def _check(logits, t, name, types, shape):
+    """A tensor beside the logits: of these types, of this shape, where the logits are, without a gradient of its own."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != logits.get_device():
         raise ValueError(f"{name} must be a tensor on {logits.device}, where the logits are")
     if t.requires_grad:
         raise ValueError(f"{name} requires grad, but gradients are computed with respect to the logits only: detach it")
+    if t.dtype not in types:
+        raise ValueError(f"{name} of type {t.dtype}: {', '.join(str(d)[6:] for d in types)} are supported")
+    if t.shape != shape:
+        raise ValueError(f"{name} of shape {tuple(t.shape)}, expected {tuple(shape)}")
+    return t
+
+
+_INTEGERS = (torch.int64, torch.int32)
+_MASKS = (torch.bool, torch.uint8)
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16, torch.float64)
 
 
 def _integers(logits, t, name, shape):
-    _same_device(logits, t, name)
-    if t.dtype not in (torch.int64, torch.int32):
-        raise ValueError(f"{name} of type {t.dtype}: int64 and int32 are supported")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} of shape {tuple(t.shape)}, expected {shape}")
-    return t.contiguous()
+    return _check(logits, t, name, _INTEGERS, shape).contiguous()
 
 
 def _mask(logits, t, shape):
-    if t is None:
-        return None
-    _same_device(logits, t, "mask")
-    if t.dtype not in (torch.bool, torch.uint8):
-        raise ValueError(f"mask of type {t.dtype}: bool and uint8 are supported")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"mask of shape {tuple(t.shape)}, expected {shape}")
-    return t.contiguous()
+    return None if t is None else _check(logits, t, "mask", _MASKS, shape).contiguous()
 
 
 def _floats(logits, t, name, shape):
-    _same_device(logits, t, name)
-    if not t.is_floating_point():
-        raise ValueError(f"{name} of type {t.dtype}: floating point is expected")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} of shape {tuple(t.shape)}, expected {shape}")
-    return t.to(torch.float32)
+    t = _check(logits, t, name, _FLOATS, shape)
+    return t if t.dtype is torch.float32 else t.to(torch.float32)
 
 
 def _row_strides(t):
@@ -132,57 +129,69 @@ def _check_out(out, logits, others):
     return out.detach()
 
 
-def _grad_like(logits):
-    """Storage for the gradient: the logits' own row strides and alignment where that wastes little memory (16-byte
-    accesses then fall on the same boundaries in both), dense rows otherwise."""
-    if logits.is_contiguous() or not logits.numel():
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+def _grad_strides(logits):
+    """Strides for a gradient's storage: the logits' own row strides where they waste little memory (16-byte accesses
+    then fall on the same boundaries in both), None for dense rows."""
+    if logits.is_contiguous():
+        return None
     reach = logits.shape[-1]
     for d in range(logits.dim() - 2, -1, -1):
         if logits.shape[d] > 1 and logits.stride(d) < reach:
-            return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)   # broadcast or reordered rows
+            return None       # broadcast or reordered rows
         reach = (logits.shape[d] - 1) * logits.stride(d) + reach
-    if reach > 1.25 * logits.numel() + 64:
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    return None if reach > 1.25 * logits.numel() + 64 else logits.stride()
+
+
+def _grad_like(logits):
+    """Storage for the gradient, aligned as the logits are."""
+    strides = _grad_strides(logits)
+    if strides is None:
+        return torch.empty_like(logits, memory_format=torch.contiguous_format)
     lead = logits.data_ptr() % 16 // logits.element_size()
-    store = torch.empty(reach + lead, dtype=logits.dtype, device=logits.device)
-    return store.as_strided(logits.shape, logits.stride(), lead)
+    reach = 1 + sum((n - 1) * s for n, s in zip(logits.shape, strides))
+    return logits.new_empty(reach + lead).as_strided(logits.shape, strides, lead)
 
 
 def _rows_of(logits, inv_temperature, grad=None):
     """The C ABI's description of the logits (and of the gradient's rows)."""
     if logits.dim() == 3:
         n_seq, n_tok, vocab = logits.shape
-        strides = (logits.stride(0), logits.stride(1))
-        gs = (grad.stride(0), grad.stride(1)) if grad is not None else (0, 0)
+        s, t, _ = logits.stride()
+        gs, gt, _ = (0, 0, 0) if grad is None else grad.stride()
     else:
         n_seq, (n_tok, vocab) = 1, logits.shape
-        strides = (0, logits.stride(0))
-        gs = (0, grad.stride(0)) if grad is not None else (0, 0)
-    return _lib.TokenLogits(logits.data_ptr(), *strides, *gs, n_seq, n_tok, vocab, _DTYPES[logits.dtype], inv_temperature)
+        s, t = 0, logits.stride(0)
+        gs, gt = 0, 0 if grad is None else grad.stride(0)
+    return _lib.TokenLogits(logits.data_ptr(), s, t, gs, gt, n_seq, n_tok, vocab, _DTYPES[logits.dtype], inv_temperature)
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)     # absent from builds of torch without a GPU
 
 
 def _call(logits, name, *args):
     """One library call on the current stream of the logits' device."""
-    dev = logits.device
-    if dev.type != "cuda":
-        raise RuntimeError(f"ppo_amd: logits on {dev}; the HIP engine has no CPU fallback")
+    index = logits.get_device()
+    if index < 0:
+        raise RuntimeError(f"ppo_amd: logits on {logits.device}; the HIP engine has no CPU fallback")
     fn = getattr(_lib.lib(), name)
-    if torch.cuda.current_device() == dev.index:
-        code = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if torch.cuda.current_device() == index:
+        code = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            code = fn(*args, torch.cuda.current_stream().cuda_stream)
-    _lib.check(code)
+        with torch.cuda.device(index):
+            code = fn(*args, _raw_stream(index))
+    if code:
+        _lib.check(code)
 
 
-def _workspace(logits):
-    n_seq, n_tok = logits.shape[:2] if logits.dim() == 3 else (1, logits.shape[0])
+def _scratch(logits, rows, floats_per_row=0):
+    """Scratch of one call and its size in bytes, behind which it has `floats_per_row` floats a row for a backward call."""
+    n_seq, n_tok = rows if len(rows) == 2 else (1, rows[0])
     need = _lib.lib().ppo_token_workspace_bytes(n_seq, n_tok)
-    return torch.empty(need, dtype=torch.uint8, device=logits.device), need
+    ws = torch.empty(need + 4 * floats_per_row * n_seq * n_tok, dtype=torch.uint8, device=logits.device)
+    return ws, need
 
 
-def _new(logits, *shape):
+def _new(logits, shape=()):
     return torch.empty(shape, dtype=torch.float32, device=logits.device)
 
 
@@ -201,19 +210,18 @@ def _written(out, logits):
 # ------------------------------------------------------------------------------------------ log-probabilities
 def _logprobs_forward(logits, tokens, mask, inv_t, entropy, stats):
     shape = logits.shape[:-1]
-    logp = _new(logits, *shape)
-    ent = _new(logits, *shape) if entropy else None
-    x = _rows_of(logits, inv_t)
-    _call(logits, "ppo_token_logprobs", ctypes.byref(x), tokens.data_ptr(), tokens.dtype == torch.int64,
-          _lib.ptr(mask), logp.data_ptr(), _lib.ptr(ent), _lib.ptr(stats))
+    logp = _new(logits, shape)
+    ent = torch.empty_like(logp) if entropy else None
+    _call(logits, "ppo_token_logprobs", ctypes.byref(_rows_of(logits, inv_t)), tokens.data_ptr(),
+          tokens.dtype is torch.int64, _lib.ptr(mask), logp.data_ptr(), _lib.ptr(ent), _lib.ptr(stats))
     return logp, ent
 
 
 def _logprobs_backward(logits, tokens, mask, inv_t, stats, g_logp, lp_strides, g_ent, ent_strides, factor):
+    """stats, g_logp, g_ent: addresses."""
     grad = _grad_like(logits)
-    x = _rows_of(logits, inv_t, grad)
-    _call(logits, "ppo_token_logprobs_backward", ctypes.byref(x), tokens.data_ptr(), tokens.dtype == torch.int64,
-          _lib.ptr(mask), stats.data_ptr(), _lib.ptr(g_logp), *lp_strides, _lib.ptr(g_ent), *ent_strides,
+    _call(logits, "ppo_token_logprobs_backward", ctypes.byref(_rows_of(logits, inv_t, grad)), tokens.data_ptr(),
+          tokens.dtype is torch.int64, _lib.ptr(mask), stats, g_logp, *lp_strides, g_ent, *ent_strides,
           _lib.ptr(factor), grad.data_ptr())
     return grad
 
@@ -223,7 +231,7 @@ class _LogprobsFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, tokens, mask, inv_t, entropy):
-        stats = _new(logits, *logits.shape[:-1], 4)
+        stats = _new(logits, (*logits.shape[:-1], 4))
         logp, ent = _logprobs_forward(logits, tokens, mask, inv_t, entropy, stats)
         ctx.inv_t = inv_t
         ctx.set_materialize_grads(False)
@@ -238,16 +246,15 @@ class _LogprobsFn(torch.autograd.Function):
         logits, tokens, mask, stats = ctx.saved_tensors
         lp_strides = _row_strides(g_logp) if g_logp is not None else (0, 0)
         ent_strides = _row_strides(g_ent) if g_ent is not None else (0, 0)
-        return (_logprobs_backward(logits, tokens, mask, ctx.inv_t, stats, g_logp, lp_strides, g_ent, ent_strides, None),
-                None, None, None, None)
+        return (_logprobs_backward(logits, tokens, mask, ctx.inv_t, stats.data_ptr(), _lib.ptr(g_logp), lp_strides,
+                                   _lib.ptr(g_ent), ent_strides, None), None, None, None, None)
 
 
 def token_logprobs(logits, tokens, mask=None, *, temperature=1.0, entropy=True):
     """Log-probability of each token and the entropy of each row's distribution: ``(logprobs, entropy)``, float32 of
     the tokens' shape (entropy is None with ``entropy=False``).  Both carry gradients to the logits; what a rollout
     needs (``[sequences, 1, vocabulary]`` or ``[sequences, vocabulary]`` logits of one step) runs under ``no_grad``."""
-    _check_logits(logits)
-    shape = tuple(logits.shape[:-1])
+    shape = _check_logits(logits)
     tokens = _integers(logits, tokens, "tokens", shape)
     mask = _mask(logits, mask, shape)
     inv_t = _temperature(temperature)
@@ -260,14 +267,13 @@ def token_logprobs(logits, tokens, mask=None, *, temperature=1.0, entropy=True):
 # ------------------------------------------------------------------------------------------ clipped policy loss
 def _policy_args(logits, tokens, old_logprobs, advantages, mask, ref_logprobs, eps_clip, eps_clip_high, kl_coef,
                  entropy_coef, temperature, reduction, scale):
-    _check_logits(logits)
-    shape = tuple(logits.shape[:-1])
+    shape = _check_logits(logits)
     tokens = _integers(logits, tokens, "tokens", shape)
     mask = _mask(logits, mask, shape)
     old = _floats(logits, old_logprobs, "old_logprobs", shape).contiguous()
-    _same_device(logits, advantages, "advantages")
-    if logits.dim() == 3 and tuple(advantages.shape) in ((shape[0],), (shape[0], 1)):
-        adv = _floats(logits, advantages, "advantages", tuple(advantages.shape))
+    per = getattr(advantages, "shape", shape)
+    if len(shape) == 2 and per != shape and per in ((shape[0],), (shape[0], 1)):
+        adv = _floats(logits, advantages, "advantages", per)
         adv_strides = (adv.stride(0), 0)
     else:
         adv = _floats(logits, advantages, "advantages", shape)
@@ -285,16 +291,19 @@ def _policy_args(logits, tokens, old_logprobs, advantages, mask, ref_logprobs, e
     return tokens, mask, old, adv, adv_strides, ref, terms, _temperature(temperature)
 
 
-def _policy_call(logits, args, stats, seeds, grad):
+def _policy_call(logits, args, grad, seeds):
+    """-> loss, log-probabilities, entropies, the scratch and where in it (bytes) lies, with `seeds`, what a backward
+    call needs: 4 floats a row of statistics, then dloss/dlogprob, then dloss/dentropy."""
     tokens, mask, old, adv, adv_strides, ref, terms, inv_t = args
-    shape = logits.shape[:-1]
-    loss, logp, ent = _new(logits), _new(logits, *shape), _new(logits, *shape)
-    ws, need = _workspace(logits)
-    x = _rows_of(logits, inv_t, grad)
-    _call(logits, "ppo_policy_loss", ctypes.byref(x), tokens.data_ptr(), tokens.dtype == torch.int64, _lib.ptr(mask),
-          old.data_ptr(), adv.data_ptr(), *adv_strides, _lib.ptr(ref), ctypes.byref(terms), loss.data_ptr(),
-          logp.data_ptr(), ent.data_ptr(), _lib.ptr(stats), _lib.ptr(seeds), _lib.ptr(grad), ws.data_ptr(), need)
-    return loss, logp, ent
+    loss, logp, ent = _new(logits), torch.empty_like(old), torch.empty_like(old)
+    ws, need = _scratch(logits, old.shape, 6 if seeds else 0)
+    at = ws.data_ptr()
+    stats = at + need if seeds else None
+    _call(logits, "ppo_policy_loss", ctypes.byref(_rows_of(logits, inv_t, grad)), tokens.data_ptr(),
+          tokens.dtype is torch.int64, _lib.ptr(mask), old.data_ptr(), adv.data_ptr(), *adv_strides, _lib.ptr(ref),
+          ctypes.byref(terms), loss.data_ptr(), logp.data_ptr(), ent.data_ptr(), stats,
+          stats + 16 * old.numel() if seeds else None, _lib.ptr(grad), at, need)
+    return loss, logp, ent, ws, need
 
 
 class _PolicyLossFn(torch.autograd.Function):
@@ -302,22 +311,21 @@ class _PolicyLossFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, args):
-        tokens, mask, *_, terms, ctx.inv_t = args
-        stats = _new(logits, *logits.shape[:-1], 4)
-        seeds = _new(logits, 2, *logits.shape[:-1])
-        loss, logp, ent = _policy_call(logits, args, stats, seeds, None)
-        ctx.with_entropy = terms.entropy_coef != 0
+        loss, logp, ent, ws, ctx.offset = _policy_call(logits, args, None, True)
+        ctx.with_entropy, ctx.inv_t = args[6].entropy_coef != 0, args[7]
+        ctx.strides, ctx.rows = _row_strides(logp), logp.numel()
         ctx.mark_non_differentiable(logp, ent)
-        ctx.save_for_backward(logits, tokens, mask, stats, seeds)
+        ctx.save_for_backward(logits, args[0], args[1], ws)
         return loss, logp, ent
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss, _g_logp, _g_ent):
-        logits, tokens, mask, stats, seeds = ctx.saved_tensors
-        strides = _row_strides(seeds[0])
-        return _logprobs_backward(logits, tokens, mask, ctx.inv_t, stats, seeds[0], strides,
-                                  seeds[1] if ctx.with_entropy else None, strides, g_loss), None
+        logits, tokens, mask, ws = ctx.saved_tensors
+        stats = ws.data_ptr() + ctx.offset
+        g_logp = stats + 16 * ctx.rows
+        return _logprobs_backward(logits, tokens, mask, ctx.inv_t, stats, g_logp, ctx.strides,
+                                  g_logp + 4 * ctx.rows if ctx.with_entropy else None, ctx.strides, g_loss), None
 
 
 def policy_loss(logits, tokens, old_logprobs, advantages, mask=None, *, ref_logprobs=None, eps_clip=0.2,
@@ -332,7 +340,7 @@ def policy_loss(logits, tokens, old_logprobs, advantages, mask=None, *, ref_logp
                         entropy_coef, temperature, reduction, scale)
     if _wants_grad(logits):
         return _PolicyLossFn.apply(logits, args)
-    return _policy_call(logits, args, None, None, None)
+    return _policy_call(logits, args, None, False)[:3]
 
 
 def policy_loss_and_grad(logits, tokens, old_logprobs, advantages, mask=None, *, ref_logprobs=None, eps_clip=0.2,
@@ -346,18 +354,17 @@ def policy_loss_and_grad(logits, tokens, old_logprobs, advantages, mask=None, *,
     grad = _grad_like(logits_) if out is None else _check_out(out, logits_, (
         ("the logits", logits_), ("tokens", args[0]), ("mask", args[1]), ("old_logprobs", args[2]),
         ("advantages", args[3]), ("ref_logprobs", args[5])))
-    loss, logp, ent = _policy_call(logits_, args, None, None, grad)
+    loss, logp, ent, _, _ = _policy_call(logits_, args, grad, False)
     _written(out, logits)
     return loss, grad, logp, ent
 
 
 # ------------------------------------------------------------------------------------------ preference loss
 def _preference_args(logits, tokens, ref_logprobs, mask, beta, label_smoothing, scale):
-    _check_logits(logits)
+    shape = _check_logits(logits)
     if logits.dim() != 3 or logits.shape[0] < 2 or logits.shape[0] % 2:
         raise ValueError("preference losses need logits [2 * pairs, tokens, vocabulary]: the preferred sequences, then "
                          f"the rejected ones in the same order; got {tuple(logits.shape)}")
-    shape = tuple(logits.shape[:-1])
     tokens = _integers(logits, tokens, "tokens", shape)
     mask = _mask(logits, mask, shape)
     ref = _floats(logits, ref_logprobs, "ref_logprobs", shape[:1]).contiguous()
@@ -366,15 +373,17 @@ def _preference_args(logits, tokens, ref_logprobs, mask, beta, label_smoothing, 
     return tokens, mask, ref, float(beta), float(label_smoothing), float(scale)
 
 
-def _preference_call(logits, args, stats, seeds, grad):
+def _preference_call(logits, args, grad, seeds):
+    """-> loss, rewards, the scratch, and with `seeds` what a backward call needs: where in the scratch the rows'
+    statistics lie (bytes), and dloss/dlogprob of each sequence's tokens."""
     tokens, mask, ref, beta, smoothing, scale = args
-    loss, rewards = _new(logits), _new(logits, logits.shape[0])
-    ws, need = _workspace(logits)
-    x = _rows_of(logits, 1.0, grad)
-    _call(logits, "ppo_preference_loss", ctypes.byref(x), tokens.data_ptr(), tokens.dtype == torch.int64,
-          _lib.ptr(mask), ref.data_ptr(), beta, smoothing, scale, loss.data_ptr(), rewards.data_ptr(), _lib.ptr(stats),
-          _lib.ptr(seeds), _lib.ptr(grad), ws.data_ptr(), need)
-    return loss, rewards
+    loss, rewards = _new(logits), torch.empty_like(ref)
+    ws, need = _scratch(logits, tokens.shape, 4 if seeds else 0)
+    at = torch.empty_like(ref) if seeds else None
+    _call(logits, "ppo_preference_loss", ctypes.byref(_rows_of(logits, 1.0, grad)), tokens.data_ptr(),
+          tokens.dtype is torch.int64, _lib.ptr(mask), ref.data_ptr(), beta, smoothing, scale, loss.data_ptr(),
+          rewards.data_ptr(), ws.data_ptr() + need if seeds else None, _lib.ptr(at), _lib.ptr(grad), ws.data_ptr(), need)
+    return loss, rewards, ws, need, at
 
 
 class _PreferenceLossFn(torch.autograd.Function):
@@ -382,17 +391,17 @@ class _PreferenceLossFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, args):
-        stats, seeds = _new(logits, *logits.shape[:-1], 4), _new(logits, logits.shape[0])
-        loss, rewards = _preference_call(logits, args, stats, seeds, None)
+        loss, rewards, ws, ctx.offset, seeds = _preference_call(logits, args, None, True)
         ctx.mark_non_differentiable(rewards)
-        ctx.save_for_backward(logits, args[0], args[1], stats, seeds)
+        ctx.save_for_backward(logits, args[0], args[1], ws, seeds)
         return loss, rewards
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss, _g_rewards):
-        logits, tokens, mask, stats, seeds = ctx.saved_tensors
-        return _logprobs_backward(logits, tokens, mask, 1.0, stats, seeds, (1, 0), None, (0, 0), g_loss), None
+        logits, tokens, mask, ws, seeds = ctx.saved_tensors
+        return _logprobs_backward(logits, tokens, mask, 1.0, ws.data_ptr() + ctx.offset, seeds.data_ptr(), (1, 0), None,
+                                  (0, 0), g_loss), None
 
 
 def preference_loss(logits, tokens, ref_logprobs, mask=None, *, beta=0.1, label_smoothing=0.0, scale=1.0):
@@ -404,7 +413,7 @@ def preference_loss(logits, tokens, ref_logprobs, mask=None, *, beta=0.1, label_
     args = _preference_args(logits, tokens, ref_logprobs, mask, beta, label_smoothing, scale)
     if _wants_grad(logits):
         return _PreferenceLossFn.apply(logits, args)
-    return _preference_call(logits, args, None, None, None)
+    return _preference_call(logits, args, None, False)[:2]
 
 
 def preference_loss_and_grad(logits, tokens, ref_logprobs, mask=None, *, beta=0.1, label_smoothing=0.0, scale=1.0,
@@ -414,41 +423,38 @@ def preference_loss_and_grad(logits, tokens, ref_logprobs, mask=None, *, beta=0.
     args = _preference_args(logits_, tokens, ref_logprobs, mask, beta, label_smoothing, scale)
     grad = _grad_like(logits_) if out is None else _check_out(out, logits_, (
         ("the logits", logits_), ("tokens", args[0]), ("mask", args[1]), ("ref_logprobs", args[2])))
-    loss, rewards = _preference_call(logits_, args, None, None, grad)
+    loss, rewards = _preference_call(logits_, args, grad, False)[:2]
     _written(out, logits)
     return loss, grad, rewards
 
 
 # ------------------------------------------------------------------------------------------ distillation
 def _distillation_args(logits, teacher_tokens, teacher_logits, mask, temperature, reduction, scale):
-    _check_logits(logits)
-    shape = tuple(logits.shape[:-1])
+    shape = _check_logits(logits)
     if not isinstance(teacher_tokens, torch.Tensor) or teacher_tokens.dim() != logits.dim() \
             or not 1 <= teacher_tokens.shape[-1] <= MAX_TEACHER_TOP:
-        raise ValueError(f"teacher_tokens must be {shape} by 1 to {MAX_TEACHER_TOP} entries")
-    full = shape + (teacher_tokens.shape[-1],)
+        raise ValueError(f"teacher_tokens must be {tuple(shape)} by 1 to {MAX_TEACHER_TOP} entries")
+    full = (*shape, teacher_tokens.shape[-1])
     index = _integers(logits, teacher_tokens, "teacher_tokens", full)
-    _same_device(logits, teacher_logits, "teacher_logits")
-    if teacher_logits.dtype not in _DTYPES:
-        raise ValueError(f"teacher_logits of type {teacher_logits.dtype}: float32, bfloat16 and float16 are supported")
-    if tuple(teacher_logits.shape) != full:
-        raise ValueError(f"teacher_logits of shape {tuple(teacher_logits.shape)}, expected {full}")
-    return (index, teacher_logits.contiguous(), _mask(logits, mask, shape), _temperature(temperature),
+    values = _check(logits, teacher_logits, "teacher_logits", _FLOATS[:3], full).contiguous()
+    return (index, values, _mask(logits, mask, shape), _temperature(temperature),
             _reduction(reduction), float(scale))
 
 
 def _teacher(index, values):
-    return index.data_ptr(), index.dtype == torch.int64, values.data_ptr(), _DTYPES[values.dtype], index.shape[-1]
+    return index.data_ptr(), index.dtype is torch.int64, values.data_ptr(), _DTYPES[values.dtype], index.shape[-1]
 
 
-def _distillation_call(logits, args, stats, grad):
+def _distillation_call(logits, args, grad, seeds):
+    """-> loss, token losses, the scratch and where in it (bytes) lie, with `seeds`, the statistics for a backward call."""
     index, values, mask, inv_t, reduction, scale = args
-    loss, each = _new(logits), _new(logits, *logits.shape[:-1])
-    ws, need = _workspace(logits)
-    x = _rows_of(logits, inv_t, grad)
-    _call(logits, "ppo_distillation_loss", ctypes.byref(x), *_teacher(index, values), _lib.ptr(mask), reduction, scale,
-          loss.data_ptr(), each.data_ptr(), _lib.ptr(stats), _lib.ptr(grad), ws.data_ptr(), need)
-    return loss, each
+    shape = logits.shape[:-1]
+    loss, each = _new(logits), _new(logits, shape)
+    ws, need = _scratch(logits, shape, 4 if seeds else 0)
+    _call(logits, "ppo_distillation_loss", ctypes.byref(_rows_of(logits, inv_t, grad)), *_teacher(index, values),
+          _lib.ptr(mask), reduction, scale, loss.data_ptr(), each.data_ptr(), ws.data_ptr() + need if seeds else None,
+          _lib.ptr(grad), ws.data_ptr(), need)
+    return loss, each, ws, need
 
 
 class _DistillationLossFn(torch.autograd.Function):
@@ -456,21 +462,19 @@ class _DistillationLossFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, args):
-        stats = _new(logits, *logits.shape[:-1], 4)
-        loss, each = _distillation_call(logits, args, stats, None)
+        loss, each, ws, ctx.offset = _distillation_call(logits, args, None, True)
         ctx.inv_t = args[3]
         ctx.mark_non_differentiable(each)
-        ctx.save_for_backward(logits, args[0], args[1], args[2], stats)
+        ctx.save_for_backward(logits, args[0], args[1], args[2], ws)
         return loss, each
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss, _g_each):
-        logits, index, values, mask, stats = ctx.saved_tensors
+        logits, index, values, mask, ws = ctx.saved_tensors
         grad = _grad_like(logits)
-        x = _rows_of(logits, ctx.inv_t, grad)
-        _call(logits, "ppo_distillation_backward", ctypes.byref(x), *_teacher(index, values), _lib.ptr(mask),
-              stats.data_ptr(), g_loss.data_ptr(), grad.data_ptr())
+        _call(logits, "ppo_distillation_backward", ctypes.byref(_rows_of(logits, ctx.inv_t, grad)),
+              *_teacher(index, values), _lib.ptr(mask), ws.data_ptr() + ctx.offset, g_loss.data_ptr(), grad.data_ptr())
         return grad, None
 
 
@@ -484,7 +488,7 @@ def distillation_loss(logits, teacher_tokens, teacher_logits, mask=None, *, temp
     args = _distillation_args(logits, teacher_tokens, teacher_logits, mask, temperature, reduction, scale)
     if _wants_grad(logits):
         return _DistillationLossFn.apply(logits, args)
-    return _distillation_call(logits, args, None, None)
+    return _distillation_call(logits, args, None, False)[:2]
 
 
 def distillation_loss_and_grad(logits, teacher_tokens, teacher_logits, mask=None, *, temperature=1.0,
@@ -495,6 +499,6 @@ def distillation_loss_and_grad(logits, teacher_tokens, teacher_logits, mask=None
     args = _distillation_args(logits_, teacher_tokens, teacher_logits, mask, temperature, reduction, scale)
     grad = _grad_like(logits_) if out is None else _check_out(out, logits_, (
         ("the logits", logits_), ("teacher_tokens", args[0]), ("teacher_logits", args[1]), ("mask", args[2])))
-    loss, each = _distillation_call(logits_, args, None, grad)
+    loss, each = _distillation_call(logits_, args, grad, False)[:2]
     _written(out, logits)
     return loss, grad, each
