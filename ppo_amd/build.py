@@ -15,6 +15,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libppo_hip.so")
 LIB_SYM = os.path.join(HERE, "libppo_hip_sym.so")
 FASTCALL = os.path.join(HERE, "_fastcall.so")          # CPython extension (csrc/fastcall.c), plain C
+TOKEN_OPS = os.path.join(HERE, "_token_ops.so")        # torch extension (csrc/token_torch.cpp), host C++
 SOURCES = ["scan.hip", "act.hip", "act_one.hip", "update.hip", "update_vjp.hip", "env.hip", "rollout.hip", "token.hip"]
 SYM_SOURCES = ["update_sym.hip"]             # + update.hip compiled with -DPPO_WITH_SYM
 HEADERS = ["ppo_common.h", "update_common.h", os.path.join("..", "..", "include", "ppo_hip.h")]
@@ -69,6 +70,29 @@ def build_fastcall(force=False, verbose=True):
     return FASTCALL
 
 
+def build_token_ops(force=False, verbose=True):
+    """The binding of ppo_amd.tokens (csrc/token_torch.cpp): host C++ against torch's headers and libraries.  It calls
+    libppo_hip.so by address and is not linked against it."""
+    import sysconfig
+    import torch
+    src = os.path.join(CSRC, "token_torch.cpp")
+    deps = [src, os.path.join(HERE, "..", "include", "ppo_hip.h"), os.path.abspath(__file__)]
+    if not force and os.path.exists(TOKEN_OPS) and all(os.path.getmtime(TOKEN_OPS) >= os.path.getmtime(d) for d in deps):
+        return TOKEN_OPS
+    at = os.path.dirname(torch.__file__)
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for inc in (os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
+                sysconfig.get_paths()["include"], "/opt/rocm/include"):
+        cmd += ["-isystem", inc]
+    cmd += [src, "-o", TOKEN_OPS, "-L" + os.path.join(at, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch",
+            "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    return TOKEN_OPS
+
+
 def build(force=False, verbose=True, variant=None, extra_flags=()):
     """Compile every HIP source for gfx950 and link the C-ABI shared libraries.  Returns the product
     library's path; build.last_action says what happened ("compiled" or "up to date").
@@ -85,6 +109,7 @@ def build(force=False, verbose=True, variant=None, extra_flags=()):
         _link([obj(s) for s in srcs], lib, verbose)
         return lib
     build_fastcall(force, verbose)
+    build_token_ops(force, verbose)
     if not force and not _stale(LIB, SOURCES) and not _stale(LIB_SYM, SOURCES + SYM_SOURCES):
         build.last_action = "up to date"
         return LIB

@@ -130,7 +130,6 @@ def test_constants_are_the_headers():
     text = open(os.path.join(os.path.dirname(_lib.HERE), "include", "ppo_hip.h")).read()
     value = lambda name: int(re.search(rf"#define {name} (\d+)", text).group(1))  # noqa: E731
     assert K.MAX_TEACHER_TOP == value("PPO_MAX_TEACHER_TOP")
-    assert K._DTYPES == {torch.float32: value("PPO_F32"), torch.bfloat16: value("PPO_BF16"), torch.float16: value("PPO_F16")}
     assert K._REDUCTIONS == {"sum": value("PPO_REDUCE_SUM"), "token_mean": value("PPO_REDUCE_TOKEN_MEAN"),
                              "sequence_mean": value("PPO_REDUCE_SEQUENCE_MEAN")}
 
@@ -220,7 +219,7 @@ def test_no_cpu_fallback(op):
 def test_gradient_storage_follows_the_logits_rows_where_that_is_cheap():
     full = torch.zeros(2, 5, 33)
     for view in (full[:, :-1], full[..., 1:], full[:, 1:]):
-        g = K._grad_like(view)
+        g = K._ops.grad_like(view)
         assert g.shape == view.shape and g.stride() == view.stride()
     for view in (full[:, -1:], torch.zeros(1, 4, 33).expand(2, 4, 33), full.transpose(0, 1), torch.zeros(2, 0, 3), full):
-        assert K._grad_like(view).is_contiguous()
+        assert K._ops.grad_like(view).is_contiguous()
