@@ -236,46 +236,45 @@ template <typename T> __device__ __forceinline__ void store_vec(T* body, int j, 
     }
 }
 
-// (m, S, E) of a row that is not kept, joined over the wave.  STREAM vectors of a thread are on their way while the
-// STREAM before are added.
-#define STREAM 4
-template <typename T, bool ENT, bool NEAR, bool KEEP>
-__device__ __forceinline__ Acc stream_stats(const T* x, int V, float c2, const Part p, float counted) {
-    constexpr int N = VEC<T>;
-    const Span<T> s(x, V);
-    const T* body = x + s.head;
-    const int e = s.edge(p.tid);
-    const float edge = e >= 0 ? wide(x[e]) : -__builtin_inff();
+// (m, S, E) of `nvec` vectors and a thread's logit of the edge (-inf: none), which are not kept, joined over the wave.
+// DEPTH vectors of a thread are on their way while the DEPTH before are added.
+template <typename T, int DEPTH, bool ENT, bool NEAR, bool KEEP>
+__device__ __forceinline__ Acc stream_stats(const T* body, int nvec, float edge, float c2, const Part& p, float counted) {
+    constexpr int N = VEC<T>, M = DEPTH < 4 ? DEPTH : 4;
     Acc a = acc_empty();
     a.n = counted;
-    if (s.nvec > 0) {
-        const int step = STREAM * p.nt, steps = s.nvec / step, left = s.nvec - steps * step;
-        u32x4 v[STREAM], next[STREAM];
+    if (nvec > 0) {
+        const int step = DEPTH * p.nt, steps = nvec / step, left = nvec - steps * step;
+        u32x4 v[DEPTH], next[DEPTH];
         const T* from = body;
         auto fetch = [&]() {          // a step of which every thread has its part
 #pragma unroll
-            for (int k = 0; k < STREAM; ++k) next[k] = load_vec<KEEP>(from + (int64_t)k * p.nt * N, p.tid);
+            for (int k = 0; k < DEPTH; ++k) next[k] = load_vec<KEEP>(from + (int64_t)k * p.nt * N, p.tid);
         };
         if (steps > 0) fetch();
         for (int i = 1; i < steps; ++i) {
             from += (int64_t)step * N;
 #pragma unroll
-            for (int k = 0; k < STREAM; ++k) v[k] = next[k];
+            for (int k = 0; k < DEPTH; ++k) v[k] = next[k];
             fetch();
             __builtin_amdgcn_sched_barrier(0);    // the loads stay ahead of the arithmetic
-            acc_vecs<T, STREAM, ENT, NEAR>(a, v, c2);
+#pragma unroll
+            for (int k = 0; k < DEPTH; k += M) acc_vecs<T, M, ENT, NEAR>(a, v + k, c2);
         }
         if (steps > 0) {
 #pragma unroll
-            for (int k = 0; k < STREAM; ++k) v[k] = next[k];
+            for (int k = 0; k < DEPTH; ++k) v[k] = next[k];
         }
         // the last step, which may be empty: threads without a part read the last vector of the row
 #pragma unroll
-        for (int k = 0; k < STREAM; ++k) next[k] = load_vec<KEEP>(body, min(steps * step + k * p.nt + p.tid, s.nvec - 1));
+        for (int k = 0; k < DEPTH; ++k) next[k] = load_vec<KEEP>(body, min(steps * step + k * p.nt + p.tid, nvec - 1));
         __builtin_amdgcn_sched_barrier(0);
-        if (steps > 0) acc_vecs<T, STREAM, ENT, NEAR>(a, v, c2);
+        if (steps > 0) {
 #pragma unroll
-        for (int k = 0; k < STREAM; ++k)
+            for (int k = 0; k < DEPTH; k += M) acc_vecs<T, M, ENT, NEAR>(a, v + k, c2);
+        }
+#pragma unroll
+        for (int k = 0; k < DEPTH; ++k)
             if (k * p.nt + p.first < left) {      // some lane of this wave has a part
                 if (k * p.nt + p.tid >= left) next[k] = Word<T>::LOWEST;
                 acc_vecs<T, 1, ENT, NEAR>(a, next + k, c2);
@@ -286,10 +285,24 @@ __device__ __forceinline__ Acc stream_stats(const T* x, int V, float c2, const P
     return acc_wave<ENT, NEAR>(a, c2);
 }
 
-// The same joined over the workgroup in its first wave: true there, and the other waves are done.
-template <typename T, bool WAVE, bool ENT, bool KEEP>
-__device__ __forceinline__ bool stream_row(const T* x, int V, float c2, float counted, Acc* lds, Acc& a) {
-    a = stream_stats<T, ENT, true, KEEP>(x, V, c2, part_of<WAVE>(), counted);
+// How a forward-only kernel reads its rows: a wave each; a workgroup each; a workgroup each where there are so few rows
+// that one's latency is what counts, with 8 vectors of a thread on their way (a row of 256 KB bf16: 12 us -> 8).
+#define MODE_WAVE 0
+#define MODE_BLOCK 1
+#define MODE_FEW 2
+
+// Part `seg` of `segs` of a row, joined over the workgroup in its first wave: true there, and the other waves are done.
+template <typename T, int MODE, bool ENT, bool KEEP>
+__device__ __forceinline__ bool stream_row(const T* x, int V, float c2, float counted, Acc* lds, Acc& a, int seg = 0,
+                                           int segs = 1) {
+    constexpr bool WAVE = MODE == MODE_WAVE;
+    const Part p = part_of<WAVE>();
+    const Span<T> s(x, V);
+    const int per = (s.nvec + segs - 1) / segs, begin = min(s.nvec, seg * per), nvec = min(per, s.nvec - begin);
+    const T* body = x + s.head + (int64_t)begin * VEC<T>;
+    const int e = seg == 0 ? s.edge(p.tid) : -1;
+    const float edge = e >= 0 ? wide(x[e]) : -__builtin_inff();
+    a = stream_stats<T, MODE == MODE_FEW ? 8 : 4, ENT, true, KEEP>(body, nvec, edge, c2, p, counted);
     if (!WAVE) {
         if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
         __syncthreads();
@@ -298,7 +311,7 @@ __device__ __forceinline__ bool stream_row(const T* x, int V, float c2, float co
     }
     const float n = a.n;
     if (is_near(a.m, c2)) a = near_done(a, c2);
-    else a = stream_stats<T, ENT, false, true>(x, V, c2, part_of<true>(), 0.0f);
+    else a = stream_stats<T, 1, ENT, false, true>(body, nvec, edge, c2, part_of<true>(), 0.0f);   // the edge is the first wave's
     a.n = n;
     return true;
 }
@@ -322,9 +335,9 @@ __device__ __forceinline__ void row_load(Row<T, CH>& row, const T* x, const Span
     }
 }
 
-template <typename T, int CH, bool WAVE, bool ENT>
-__device__ __forceinline__ Acc row_stats(Row<T, CH>& row, const T* x, const Span<T>& s, const Part& p, float c2,
-                                         float counted, Acc* lds) {
+// A thread's part of (m, S, E), joined over the wave, in the NEAR form.
+template <typename T, int CH, bool ENT>
+__device__ __forceinline__ Acc row_stats(Row<T, CH>& row, const T* x, const Span<T>& s, const Part& p, float c2, float counted) {
     constexpr int M = sizeof(T) == 4 ? 4 : 2;             // vectors added at once
     const int mine = s.nvec - p.first;
     Acc a = acc_empty();
@@ -335,17 +348,24 @@ __device__ __forceinline__ Acc row_stats(Row<T, CH>& row, const T* x, const Span
 #pragma unroll
             for (int k = i; k < i + M; ++k)
                 if (k * p.nt + 64 > mine && k * p.nt + p.tid >= s.nvec) row.v[k] = Word<T>::LOWEST;
-            acc_vecs<T, M, ENT>(a, row.v + i, c2);
+            acc_vecs<T, M, ENT, true>(a, row.v + i, c2);
         }
     }
     if (CH == 16)
         for (int j = CH * p.nt + p.tid; j < s.nvec; j += p.nt) {
             const u32x4 v = load_vec<true>(x + s.head, j);
-            acc_vecs<T, 1, ENT>(a, &v, c2);
+            acc_vecs<T, 1, ENT, true>(a, &v, c2);
         }
-    acc_rebase<ENT>(a, fmaxf(a.m, row.edge), c2);
-    acc_add<ENT>(a, row.edge, c2);
-    a = acc_wave<ENT>(a, c2);
+    acc_rebase<ENT, true>(a, fmaxf(a.m, row.edge), c2);
+    acc_add<ENT, true>(a, row.edge, c2);
+    return acc_wave<ENT, true>(a, c2);
+}
+
+// The exact statistics of a row that is not near, by all of its threads and in all of them.
+template <typename T, bool WAVE, bool ENT>
+__device__ __forceinline__ Acc far_stats(const T* x, const Span<T>& s, const Part& p, float c2, Acc* lds) {
+    const int e = s.edge(p.tid);
+    Acc a = stream_stats<T, 1, ENT, false, true>(x + s.head, s.nvec, e >= 0 ? wide(x[e]) : -__builtin_inff(), c2, p, 0.0f);
     if (WAVE) return a;
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
     __syncthreads();
@@ -353,25 +373,25 @@ __device__ __forceinline__ Acc row_stats(Row<T, CH>& row, const T* x, const Span
 }
 
 // ------------------------------------------------------------------------------------------ row gradient
-// dL/dx_i = e_i (a + b u_i), + gt at `tok`
+// dL/dx_i = e_i (a + b u_i), + gt at `tok`; u_i = fma(x_i, c2, -m) in the NEAR form, (x_i - m) c2 in the other
 struct RowGrad {
     float m, a, b, gt;
     int tok;     // -1: none
 };
 
-template <bool ENT> __device__ __forceinline__ float grad_of(const RowGrad& g, float x, float c2) {
-    const float u = (x - g.m) * c2;
+template <bool ENT, bool NEAR> __device__ __forceinline__ float grad_of(const RowGrad& g, float x, float c2) {
+    const float u = NEAR ? fmaf(x, c2, -g.m) : (x - g.m) * c2;
     const float e = __builtin_amdgcn_exp2f(u);
     return ENT ? e * fmaf(g.b, fmaxf(u, U_FLOOR), g.a) : e * g.a;
 }
 
-template <typename T, bool ENT>
+template <typename T, bool ENT, bool NEAR>
 __device__ __forceinline__ u32x4 grad_vec(const RowGrad& g, u32x4 v, int place, float c2) {   // place: of the token in v
     constexpr int N = VEC<T>;
     float d[N];
     unpack<T>(v, d);
 #pragma unroll
-    for (int i = 0; i < N; ++i) d[i] = grad_of<ENT>(g, d[i], c2);
+    for (int i = 0; i < N; ++i) d[i] = grad_of<ENT, NEAR>(g, d[i], c2);
     if (place >= 0 && place < N) {
 #pragma unroll
         for (int i = 0; i < N; ++i) d[i] += i == place ? g.gt : 0.0f;
@@ -379,14 +399,14 @@ __device__ __forceinline__ u32x4 grad_vec(const RowGrad& g, u32x4 v, int place, 
     return pack<T>(d);        // the one rounding of the gradient
 }
 
-template <typename T, bool ENT>
+template <typename T, bool ENT, bool NEAR>
 __device__ __forceinline__ void edge_grad(const RowGrad& g, float x, T* out, int i, float c2) {
     if (i < 0) return;
-    const float d = grad_of<ENT>(g, x, c2);
+    const float d = grad_of<ENT, NEAR>(g, x, c2);
     out[i] = (T)(i == g.tok ? d + g.gt : d);
 }
 
-// The gradient of a held row.  The vectors that are read again may lie where their gradient goes.
+// The gradient of a held row that is near.  The vectors that are read again may lie where their gradient goes.
 template <typename T, int CH, bool ENT>
 __device__ __forceinline__ void row_grad(const Row<T, CH>& row, const T* x, T* out, const Span<T>& s, const Part& p,
                                          float c2, const RowGrad& g, bool past) {
@@ -397,17 +417,17 @@ __device__ __forceinline__ void row_grad(const Row<T, CH>& row, const T* x, T* o
     for (int i = 0; i < CH; ++i) {
         if (i * p.nt < mine) {
             const int j = i * p.nt + p.tid;
-            const u32x4 o = grad_vec<T, ENT>(g, row.v[i], tok - j * N, c2);
+            const u32x4 o = grad_vec<T, ENT, true>(g, row.v[i], tok - j * N, c2);
             if (j < s.nvec) store_vec(out + s.head, j, o, past);
         }
     }
     if (CH == 16)
         for (int j = CH * p.nt + p.tid; j < s.nvec; j += p.nt)
-            store_vec(out + s.head, j, grad_vec<T, ENT>(g, load_vec<false>(x + s.head, j), tok - j * N, c2), past);
-    edge_grad<T, ENT>(g, row.edge, out, s.edge(p.tid), c2);
+            store_vec(out + s.head, j, grad_vec<T, ENT, true>(g, load_vec<false>(x + s.head, j), tok - j * N, c2), past);
+    edge_grad<T, ENT, true>(g, row.edge, out, s.edge(p.tid), c2);
 }
 
-// The gradient of a row whose statistics are known, vectors j0 up to j1; x may be out.
+// The gradient of a row whose statistics are known, part `seg` of `segs`; x may be out.
 template <typename T, bool ENT>
 __device__ __forceinline__ void row_map(const T* x, T* out, int V, const Part& p, int seg, int segs, float c2,
                                         const RowGrad& g, bool past) {
@@ -416,9 +436,9 @@ __device__ __forceinline__ void row_map(const T* x, T* out, int V, const Part& p
     const int per = (s.nvec + segs - 1) / segs, end = min(s.nvec, (seg + 1) * per);
     const int tok = g.tok >= 0 ? g.tok - s.head : -1;
     for (int j = seg * per + p.tid; j < end; j += p.nt)
-        store_vec(out + s.head, j, grad_vec<T, ENT>(g, load_vec<false>(x + s.head, j), tok - j * N, c2), past);
+        store_vec(out + s.head, j, grad_vec<T, ENT, false>(g, load_vec<false>(x + s.head, j), tok - j * N, c2), past);
     const int e = seg == 0 ? s.edge(p.tid) : -1;
-    edge_grad<T, ENT>(g, e >= 0 ? wide(x[e]) : 0.0f, out, e, c2);
+    edge_grad<T, ENT, false>(g, e >= 0 ? wide(x[e]) : 0.0f, out, e, c2);
 }
 
 template <typename T> __device__ __forceinline__ void row_fill(T* out, int V, const Part& p, int seg, int segs, bool past) {
@@ -588,10 +608,11 @@ __global__ __launch_bounds__(1024) void total_kernel(const double* __restrict__ 
 }
 
 // ------------------------------------------------------------------------------------------ log-probabilities
-template <typename T, bool WAVE, bool ENT, bool KEEP>
+template <typename T, int MODE, bool ENT, bool KEEP>
 __global__ __launch_bounds__(1024, 4) void logprobs_kernel(Logits L, const void* tokens, int i64, const uint8_t* mask,
                                                            float* logprobs, double* logprobs64, float* entropy,
                                                            RowStats* stats) {
+    constexpr bool WAVE = MODE == MODE_WAVE;
     __shared__ Acc lds[16];
     const int64_t r = row_of<WAVE>(L);
     if (WAVE && r >= L.n) return;
@@ -601,7 +622,7 @@ __global__ __launch_bounds__(1024, 4) void logprobs_kernel(Logits L, const void*
         const T* x = row_in<T>(L, place_of(L, r));
         const float xt = token_logit(x, int_at(tokens, i64, r), L.V);
         Acc a;
-        if (!stream_row<T, WAVE, ENT, KEEP>(x, L.V, L.c2, 0.0f, lds, a)) return;
+        if (!stream_row<T, MODE, ENT, KEEP>(x, L.V, L.c2, 0.0f, lds, a)) return;
         const double ln_s = ln_of(a.s);
         lp = logp_of(xt, L.c, a, ln_s);
         st.m = a.m;
@@ -733,53 +754,70 @@ template <bool WAVE> __device__ __forceinline__ void row_loss(const PolicyArgs& 
     if (threadIdx.x == 0) *p.solo = (float)loss;
 }
 
+// A counted row from its statistics to what the loss and its gradient need of it.
+struct PolicyDone {
+    double lp, ln_s;
+    float h;
+    PolicyRow o;
+};
+__device__ __forceinline__ PolicyDone policy_done(const Logits& L, const PolicyArgs& p, const PolicyIn& in, const Acc& a,
+                                                  const Place& at, float counted) {
+    PolicyDone d;
+    d.ln_s = ln_of(a.s);
+    d.lp = logp_of(in.xt, L.c, a, d.ln_s);
+    d.h = entropy_of(a, d.ln_s);
+    d.o = policy_row(p, d.lp, d.h, in.old_lp, in.adv, in.ref, row_weight(p.w, at, L.n_tok, counted));
+    return d;
+}
+
 // Forward only; leaves what the backward pass needs.
-template <typename T, bool WAVE>
+template <typename T, int MODE>
 __global__ __launch_bounds__(1024, 4) void policy_forward_kernel(Logits L, PolicyArgs p) {
+    constexpr bool WAVE = MODE == MODE_WAVE;
     __shared__ Acc lds[16];
     const int64_t r = row_of<WAVE>(L);
-    PolicyRow o = {0.0, 0.0f, 0.0f};
+    PolicyDone d = {0.0, 0.0, 0.0f, {0.0, 0.0f, 0.0f}};
     if (!WAVE || r < L.n) {
         RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
-        double lp = 0.0;
         if (!p.w.mask || p.w.mask[r]) {
             const Place at = place_of(L, r);
             const T* x = row_in<T>(L, at);
             const PolicyIn in = policy_in(L, p, x, r, at);
             Acc a;
-            if (!stream_row<T, WAVE, true, true>(x, L.V, L.c2, count_mask(p.w, L.n, part_of<WAVE>()), lds, a)) return;
-            const double ln_s = ln_of(a.s);
-            lp = logp_of(in.xt, L.c, a, ln_s);
-            st.m = a.m;
-            st.s = a.s;
-            st.h = entropy_of(a, ln_s);
-            o = policy_row(p, lp, st.h, in.old_lp, in.adv, in.ref, row_weight(p.w, at, L.n_tok, a.n));
+            if (!stream_row<T, MODE, true, true>(x, L.V, L.c2, count_mask(p.w, L.n, part_of<WAVE>()), lds, a)) return;
+            d = policy_done(L, p, in, a, at, a.n);
+            st = {a.m, a.s, d.h, 0.0f};
         }
         if (part_of<WAVE>().tid == 0) {
-            p.logprobs[r] = (float)lp;
-            if (p.entropy) p.entropy[r] = st.h;
+            p.logprobs[r] = (float)d.lp;
+            if (p.entropy) p.entropy[r] = d.h;
             if (p.stats) {
                 p.stats[r] = st;
-                p.g_lp[r] = o.g_lp;
-                p.g_h[r] = o.g_h;
+                p.g_lp[r] = d.o.g_lp;
+                p.g_h[r] = d.o.g_h;
             }
         }
     }
-    row_loss<WAVE>(p, r, L.n, o.loss);
+    row_loss<WAVE>(p, r, L.n, d.o.loss);
 }
 
-// Loss and gradient: the row stays on the chip between its statistics and its gradient.
+// Loss and gradient: the row stays on the chip between its statistics and its gradient.  The first wave makes of the
+// statistics what all others need (a row's fp64 arithmetic is some 300 instructions, as much as 30 vectors' gradient).
+struct RowShared {
+    Acc acc[16];
+    RowGrad grad;
+    int near_;
+};
+
 template <typename T, int CH, bool WAVE, bool ENT_GRAD>
 __global__ __launch_bounds__(1024, 4) void policy_kernel(Logits L, PolicyArgs p) {
-    __shared__ Acc lds[16];
+    __shared__ RowShared sh;
     const Part q = part_of<WAVE>();
     const int64_t r = row_of<WAVE>(L);
-    double loss = 0.0;
+    PolicyDone d = {0.0, 0.0, 0.0f, {0.0, 0.0f, 0.0f}};
     if (!WAVE || r < L.n) {
         const Place at = place_of(L, r);
         T* out = row_out<T>(L, at);
-        double lp = 0.0;
-        float h = 0.0f;
         if (!p.w.mask || p.w.mask[r]) {
             const T* x = row_in<T>(L, at);
             const Span<T> s(x, L.V);
@@ -787,24 +825,118 @@ __global__ __launch_bounds__(1024, 4) void policy_kernel(Logits L, PolicyArgs p)
             const PolicyIn in = policy_in(L, p, x, r, at);
             row_load(row, x, s, q);
             const float counted = count_mask(p.w, L.n, q);
-            asm volatile("" :: "v"(in.xt));   // read before the barrier in row_stats: the gradient may overwrite it
-            const Acc a = row_stats<T, CH, WAVE, true>(row, x, s, q, L.c2, counted, lds);
-            const double ln_s = ln_of(a.s);
-            lp = logp_of(in.xt, L.c, a, ln_s);
-            h = entropy_of(a, ln_s);
-            const PolicyRow o = policy_row(p, lp, h, in.old_lp, in.adv, in.ref, row_weight(p.w, at, L.n_tok, a.n));
-            loss = o.loss;
-            row_grad<T, CH, ENT_GRAD>(row, x, out, s, q, L.c2, grad_seed(a.m, a.s, h, o.g_lp, o.g_h, in.tok, L.V, L.c),
-                                      L.past);
+            asm volatile("" :: "v"(in.xt));   // read before the barrier: the gradient may overwrite it
+            Acc a = row_stats<T, CH, true>(row, x, s, q, L.c2, counted);
+            RowGrad g;
+            bool near_ = true;
+            if (!WAVE) {
+                if ((threadIdx.x & 63) == 0) sh.acc[threadIdx.x >> 6] = a;
+                __syncthreads();
+            }
+            if (WAVE || q.first == 0) {
+                if (!WAVE) a = acc_waves<true, true>(sh.acc, L.c2);
+                near_ = is_near(a.m, L.c2);
+                d = policy_done(L, p, in, near_done(a, L.c2), at, a.n);
+                g = grad_seed(near_max(a.m, L.c2), a.s, d.h, d.o.g_lp, d.o.g_h, in.tok, L.V, L.c);
+                if (!WAVE && threadIdx.x == 0) {
+                    sh.grad = g;
+                    sh.near_ = near_;
+                }
+            }
+            if (!WAVE) {
+                __syncthreads();
+                g = sh.grad;
+                near_ = sh.near_;
+            }
+            if (near_) {
+                row_grad<T, CH, ENT_GRAD>(row, x, out, s, q, L.c2, g, L.past);
+            } else {
+                const float n = a.n;
+                a = far_stats<T, WAVE, true>(x, s, q, L.c2, sh.acc);
+                d = policy_done(L, p, in, a, at, n);      // (n: the first wave's, which alone uses the weighted results)
+                if (!WAVE) {
+                    if (threadIdx.x == 0) sh.grad = grad_seed(a.m, a.s, d.h, d.o.g_lp, d.o.g_h, in.tok, L.V, L.c);
+                    __syncthreads();
+                    g = sh.grad;
+                } else {
+                    g = grad_seed(a.m, a.s, d.h, d.o.g_lp, d.o.g_h, in.tok, L.V, L.c);
+                }
+                row_map<T, ENT_GRAD>(x, out, L.V, q, 0, 1, L.c2, g, L.past);
+            }
         } else {
             row_fill(out, L.V, q, 0, 1, L.past);
         }
         if (q.tid == 0) {
-            p.logprobs[r] = (float)lp;
-            if (p.entropy) p.entropy[r] = h;
+            p.logprobs[r] = (float)d.lp;
+            if (p.entropy) p.entropy[r] = d.h;
         }
     }
-    row_loss<WAVE>(p, r, L.n, loss);
+    row_loss<WAVE>(p, r, L.n, d.o.loss);
+}
+
+// Few long rows: a row in `parts` pieces of a workgroup each, first their statistics (split_stats_kernel), then, in a
+// second launch, the row's loss and the pieces' gradients.  The first launch also takes along what of the logits the
+// second needs beside its piece, which another workgroup of that launch may have overwritten.
+#define SPLIT_PARTS 64
+struct Split {
+    Acc* acc;                 // n * parts; n of a row's first one: the token's logit
+    int* teach;               // entries of each row (distillation)
+    int parts;
+};
+
+template <typename T, bool ENT>
+__global__ __launch_bounds__(256) void split_stats_kernel(Logits L, const uint8_t* mask, const void* tokens, int i64, Split sp) {
+    __shared__ Acc lds[16];
+    const int64_t r = blockIdx.x;
+    if (mask && !mask[r]) return;
+    const T* x = row_in<T>(L, place_of(L, r));
+    const float xt = tokens && blockIdx.y == 0 ? token_logit(x, int_at(tokens, i64, r), L.V) : 0.0f;
+    Acc a;
+    if (!stream_row<T, MODE_BLOCK, ENT, true>(x, L.V, L.c2, 0.0f, lds, a, blockIdx.y, sp.parts)) return;
+    a.n = xt;
+    if (threadIdx.x == 0) sp.acc[r * sp.parts + blockIdx.y] = a;
+}
+
+// A row's pieces joined, by a wave and in all of its lanes.
+template <bool ENT> __device__ __forceinline__ Acc split_join(const Split& sp, int64_t r, float c2) {
+    const int lane = threadIdx.x & 63;
+    Acc a = acc_empty();
+    if (lane < sp.parts) a = sp.acc[r * sp.parts + lane];
+    a.n = 0.0f;
+    return acc_wave<ENT>(a, c2);
+}
+
+template <typename T, bool ENT_GRAD>
+__global__ __launch_bounds__(256) void policy_split_kernel(Logits L, PolicyArgs p, Split sp) {
+    __shared__ RowShared sh;
+    const Part q = part_of<false>();
+    const int64_t r = blockIdx.x;
+    const Place at = place_of(L, r);
+    T* out = row_out<T>(L, at);
+    PolicyDone d = {0.0, 0.0, 0.0f, {0.0, 0.0f, 0.0f}};
+    if (!p.w.mask || p.w.mask[r]) {
+        if (q.first == 0) {
+            PolicyIn in;
+            in.tok = int_at(p.tokens, p.i64, r);
+            in.old_lp = p.old_lp[r];
+            in.adv = p.adv[at.b * p.adv_s + at.t * p.adv_t];
+            in.ref = p.ref ? p.ref[r] : 0.0f;
+            in.xt = sp.acc[r * sp.parts].n;
+            const Acc a = split_join<true>(sp, r, L.c2);
+            d = policy_done(L, p, in, a, at, wave_sum(count_mask(p.w, L.n, part_of<true>())));
+            if (threadIdx.x == 0) sh.grad = grad_seed(a.m, a.s, d.h, d.o.g_lp, d.o.g_h, in.tok, L.V, L.c);
+        }
+        __syncthreads();
+        row_map<T, ENT_GRAD>(row_in<T>(L, at), out, L.V, q, blockIdx.y, gridDim.y, L.c2, sh.grad, L.past);
+    } else {
+        row_fill(out, L.V, q, blockIdx.y, gridDim.y, L.past);
+    }
+    if (blockIdx.y > 0) return;
+    if (threadIdx.x == 0) {
+        p.logprobs[r] = (float)d.lp;
+        if (p.entropy) p.entropy[r] = d.h;
+    }
+    row_loss<false>(p, r, L.n, d.o.loss);
 }
 
 // ------------------------------------------------------------------------------------------ preference loss
@@ -867,6 +999,7 @@ struct Teacher {
         : index(lds + 2), q((float*)(lds + 2 + K)), x((float*)(lds + 2 + 2 * K)), bad(lds), some(lds + 1) {}
 };
 static size_t teacher_lds(int K) { return (size_t)(2 + 3 * K) * 4; }
+#define TEACHER_WORDS (4 + 3 * PPO_MAX_TEACHER_TOP)      // the same of a row in memory: bad, some, sum q ln q, then the arrays
 
 // First wave only.  Returns sum q ln q.
 template <typename T>
@@ -920,21 +1053,26 @@ __device__ __forceinline__ RowGrad teacher_seed(const Teacher& s, float m, float
     return {m, *s.bad ? __builtin_nanf("") : *s.some ? g / sum : 0.0f, 0.0f, 0.0f, -1};
 }
 
-template <typename T>
+template <typename T, bool NEAR>
 __device__ __forceinline__ void teacher_places(const TeacherArgs& p, const Teacher& s, T* out, const Logits& L,
-                                               const RowGrad& rg, float g) {
+                                               const RowGrad& rg, float g, const Span<T>& w, int seg = 0, int segs = 1) {
     __syncthreads();          // the bulk is written
     if (*s.bad) return;
+    const int per = (w.nvec + segs - 1) / segs;
     for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
         const int i = s.index[k];
         if (i < 0) continue;
+        if (segs > 1) {       // of this piece only; the edge is the first one's
+            const int j = i < w.head ? -1 : (i - w.head) / VEC<T>;
+            if ((j < 0 || j >= w.nvec ? 0 : j / per) != seg) continue;
+        }
         float all = 0.0f;     // a token that appears twice: both entries, in both places the same number
         for (int j = 0; j < p.K; ++j) all += s.index[j] == i ? s.q[j] : 0.0f;
-        out[i] = (T)(grad_of<false>(rg, s.x[k], L.c2) - g * all);
+        out[i] = (T)(grad_of<false, NEAR>(rg, s.x[k], L.c2) - g * all);
     }
 }
 
-template <typename T>
+template <typename T, int MODE>
 __global__ __launch_bounds__(1024, 4) void distill_forward_kernel(Logits L, TeacherArgs p) {
     __shared__ Acc lds[16];
     extern __shared__ int entries[];
@@ -948,7 +1086,7 @@ __global__ __launch_bounds__(1024, 4) void distill_forward_kernel(Logits L, Teac
         float ent = 0.0f;
         if (threadIdx.x < 64) ent = teacher_load(p, L, r, x, teach);
         Acc a;
-        if (!stream_row<T, false, false, true>(x, L.V, L.c2, count_mask(p.w, L.n, part_of<false>()), lds, a)) return;
+        if (!stream_row<T, MODE, false, true>(x, L.V, L.c2, count_mask(p.w, L.n, part_of<false>()), lds, a)) return;
         loss = teacher_loss(p, teach, ent, a, L.c) / (L.c * L.c);
         st.m = a.m;
         st.s = a.s;
@@ -964,7 +1102,7 @@ __global__ __launch_bounds__(1024, 4) void distill_forward_kernel(Logits L, Teac
 
 template <typename T, int CH>
 __global__ __launch_bounds__(1024, 4) void distill_kernel(Logits L, TeacherArgs p) {
-    __shared__ Acc lds[16];
+    __shared__ RowShared sh;
     extern __shared__ int entries[];
     const Teacher teach(entries, p.K);
     const int64_t r = row_of<false>(L);
@@ -979,11 +1117,24 @@ __global__ __launch_bounds__(1024, 4) void distill_kernel(Logits L, TeacherArgs 
         row_load(row, x, s, q);
         float ent = 0.0f;
         if (q.first == 0) ent = teacher_load(p, L, r, x, teach);
-        const Acc a = row_stats<T, CH, false, false>(row, x, s, q, L.c2, count_mask(p.w, L.n, q), lds);
+        Acc a = row_stats<T, CH, false>(row, x, s, q, L.c2, count_mask(p.w, L.n, q));
+        if ((threadIdx.x & 63) == 0) sh.acc[threadIdx.x >> 6] = a;
+        __syncthreads();
+        a = acc_waves<false, true>(sh.acc, L.c2);
         w = row_weight(p.w, at, L.n_tok, a.n);
-        const RowGrad g = teacher_seed(teach, a.m, a.s, w / L.c);
-        row_grad<T, CH, false>(row, x, out, s, q, L.c2, g, L.past);
-        teacher_places(p, teach, out, L, g, w / L.c);
+        const float scale = w / L.c;
+        if (is_near(a.m, L.c2)) {
+            const RowGrad g = teacher_seed(teach, near_max(a.m, L.c2), a.s, scale);
+            row_grad<T, CH, false>(row, x, out, s, q, L.c2, g, L.past);
+            teacher_places<T, true>(p, teach, out, L, g, scale, s);
+            a = near_done(a, L.c2);
+        } else {
+            __syncthreads();  // sh.acc has been read
+            a = far_stats<T, false, false>(x, s, q, L.c2, sh.acc);
+            const RowGrad g = teacher_seed(teach, a.m, a.s, scale);
+            row_map<T, false>(x, out, L.V, q, 0, 1, L.c2, g, L.past);
+            teacher_places<T, false>(p, teach, out, L, g, scale, s);
+        }
         if (q.first == 0) loss = teacher_loss(p, teach, ent, a, L.c) / (L.c * L.c);
     } else {
         row_fill(out, L.V, q, 0, 1, L.past);
@@ -993,6 +1144,54 @@ __global__ __launch_bounds__(1024, 4) void distill_kernel(Logits L, TeacherArgs 
         if (p.solo) *p.solo = (float)((double)w * (double)loss);
         else p.part[r] = (double)w * (double)loss;
     }
+}
+
+// Few long rows, as policy_split_kernel: the teacher's entries are made by a workgroup of their own beside the pieces'
+// statistics, because another piece's gradient may lie where the policy's logits of the entries were.
+template <typename T> __global__ __launch_bounds__(64) void split_teacher_kernel(Logits L, TeacherArgs p, Split sp) {
+    extern __shared__ int entries[];
+    const Teacher teach(entries, p.K);
+    const int64_t r = blockIdx.x;
+    if (p.w.mask && !p.w.mask[r]) return;
+    const float ent = teacher_load(p, L, r, row_in<T>(L, place_of(L, r)), teach);
+    __syncthreads();
+    int* to = sp.teach + r * TEACHER_WORDS;
+    for (int k = threadIdx.x; k < 2 + 3 * p.K; k += 64) to[k < 2 ? k : k + 2] = entries[k];
+    if (threadIdx.x == 0) to[2] = __float_as_int(ent);
+}
+
+template <typename T> __global__ __launch_bounds__(256) void distill_split_kernel(Logits L, TeacherArgs p, Split sp) {
+    extern __shared__ int entries[];
+    __shared__ Acc joined;
+    const Teacher teach(entries, p.K);
+    const int64_t r = blockIdx.x;
+    const Part q = part_of<false>();
+    const Place at = place_of(L, r);
+    T* out = row_out<T>(L, at);
+    float loss = 0.0f, w = 0.0f;
+    if (!p.w.mask || p.w.mask[r]) {
+        const int* from = sp.teach + r * TEACHER_WORDS;
+        for (int k = threadIdx.x; k < 2 + 3 * p.K; k += 256) entries[k] = from[k < 2 ? k : k + 2];
+        if (q.first == 0) {
+            Acc a = split_join<false>(sp, r, L.c2);
+            a.n = wave_sum(count_mask(p.w, L.n, part_of<true>()));
+            if (threadIdx.x == 0) joined = a;
+        }
+        __syncthreads();
+        const Acc a = joined;
+        w = row_weight(p.w, at, L.n_tok, a.n);
+        const T* x = row_in<T>(L, at);
+        const RowGrad g = teacher_seed(teach, a.m, a.s, w / L.c);
+        row_map<T, false>(x, out, L.V, q, blockIdx.y, gridDim.y, L.c2, g, L.past);
+        teacher_places<T, false>(p, teach, out, L, g, w / L.c, Span<T>(x, L.V), blockIdx.y, gridDim.y);
+        if (q.first == 0) loss = teacher_loss(p, teach, __int_as_float(from[2]), a, L.c) / (L.c * L.c);
+    } else {
+        row_fill(out, L.V, q, blockIdx.y, gridDim.y, L.past);
+    }
+    if (threadIdx.x > 0 || blockIdx.y > 0) return;
+    if (p.losses) p.losses[r] = loss;
+    if (p.solo) *p.solo = (float)((double)w * (double)loss);
+    else p.part[r] = (double)w * (double)loss;
 }
 
 template <typename T> __global__ __launch_bounds__(256) void distill_backward_kernel(Logits L, TeacherArgs p) {
@@ -1013,13 +1212,14 @@ template <typename T> __global__ __launch_bounds__(256) void distill_backward_ke
     const float g = (p.factor ? *p.factor : 1.0f) * st.w / L.c;
     const RowGrad rg = teacher_seed(teach, st.m, st.s, g);
     row_map<T, false>(x, out, L.V, q, 0, 1, L.c2, rg, L.past);
-    teacher_places(p, teach, out, L, rg, g);
+    teacher_places<T, false>(p, teach, out, L, rg, g, Span<T>(x, L.V));
 }
 
 // ------------------------------------------------------------------------------------------ host side
 #define ALIGN256(n) (((size_t)(n) + 255) & ~(size_t)255)
 
 #define TOTAL_GRID 64
+#define SPLIT_ROWS 128
 
 struct Workspace {            // one call's scratch
     double *part, *sums;      // weighted loss of each row (or pair); TOTAL_GRID sums of them
@@ -1027,6 +1227,8 @@ struct Workspace {            // one call's scratch
     double* lp64;             // the pairs' log-probabilities
     float* seeds;             // and their gradients
     RowStats* stats;
+    Acc* acc;                 // statistics of pieces of few long rows
+    int* teach;               // and their teacher's entries
     size_t bytes;
 };
 
@@ -1041,6 +1243,9 @@ static Workspace carve(void* base, int64_t n_seq, int64_t n_tok) {
     w.lp64 = (double*)take(8 * (size_t)(n_seq * n_tok));
     w.seeds = (float*)take(4 * (size_t)n_seq);
     w.stats = (RowStats*)take(sizeof(RowStats) * (size_t)(n_seq * n_tok));
+    const size_t few = (size_t)(n_seq * n_tok < SPLIT_ROWS ? n_seq * n_tok : SPLIT_ROWS);
+    w.acc = (Acc*)take(sizeof(Acc) * few * SPLIT_PARTS);
+    w.teach = (int*)take(4 * few * TEACHER_WORDS);
     w.bytes = (size_t)(p - (char*)base);
     return w;
 }
@@ -1114,7 +1319,20 @@ static bool by_wave(const Logits& L, int dtype) { return row_bytes(L, dtype) <= 
 
 // Threads of a row that is only read: few, because what is done once a row costs each wave the same, and the chip is
 // full with 256 rows under way and more; all that a workgroup can have where there are fewer rows than that.
-static int stream_threads(const Logits& L) { return L.n >= 512 ? 256 : 1024; }
+static int stream_mode(const Logits& L, int dtype) { return by_wave(L, dtype) ? MODE_WAVE : L.n >= 512 ? MODE_BLOCK : MODE_FEW; }
+static int stream_threads(int mode) { return mode == MODE_FEW ? 1024 : 256; }
+#define BY_MODE(mode, M, ...)                                                      \
+    if ((mode) == MODE_WAVE) { constexpr int M = MODE_WAVE; __VA_ARGS__; }         \
+    else if ((mode) == MODE_BLOCK) { constexpr int M = MODE_BLOCK; __VA_ARGS__; }  \
+    else { constexpr int M = MODE_FEW; __VA_ARGS__; }
+
+// Pieces of a row where there are so few long ones that they leave most of the chip idle; 0: the row is not cut.
+static int split_parts(const Logits& L, int dtype) {
+    if (L.n > SPLIT_ROWS || row_bytes(L, dtype) < 65536) return 0;
+    const int64_t most = row_bytes(L, dtype) / 8192, want = 1024 / L.n;
+    const int64_t parts = want < most ? want : most;
+    return (int)(parts < SPLIT_PARTS ? parts : SPLIT_PARTS);
+}
 
 // Threads of a row that is held in CH vectors each: as many as it needs.
 static int held_threads(const Logits& L, int dtype, int CH) {
@@ -1156,8 +1374,8 @@ static int weights_of(Weights* o, const uint8_t* mask, int reduction, float scal
 
 static void launch_logprobs(Logits L, int dtype, const void* tokens, int i64, const uint8_t* mask, float* logprobs,
                             double* logprobs64, float* entropy, RowStats* stats, hipStream_t st) {
-    BY_TYPE(dtype, T, BY_FLAG(by_wave(L, dtype), WAVE, BY_FLAG(entropy != nullptr, ENT, BY_FLAG(stats != nullptr, KEEP, {
-        EACH_LAUNCH(L, WAVE, grid, (logprobs_kernel<T, WAVE, ENT, KEEP><<<grid, WAVE ? 256 : stream_threads(L), 0, st>>>(
+    BY_TYPE(dtype, T, BY_MODE(stream_mode(L, dtype), MODE, BY_FLAG(entropy != nullptr, ENT, BY_FLAG(stats != nullptr, KEEP, {
+        EACH_LAUNCH(L, MODE == MODE_WAVE, grid, (logprobs_kernel<T, MODE, ENT, KEEP><<<grid, stream_threads(MODE), 0, st>>>(
             L, tokens, i64, mask, logprobs, logprobs64, entropy, stats)))
     }))))
 }
@@ -1244,8 +1462,16 @@ extern "C" int ppo_policy_loss(const ppo_token_logits* x, const void* tokens, in
         p.solo = solo ? loss : nullptr;
         count_rows(p.w, x, w, st);
         if (!grad) {
-            BY_TYPE(x->dtype, T, BY_FLAG(by_wave(L, x->dtype), WAVE, {
-                EACH_LAUNCH(L, WAVE, grid, (policy_forward_kernel<T, WAVE><<<solo ? 1 : grid, WAVE ? solo ? 64 * (int)L.n : 256 : stream_threads(L), 0, st>>>(L, p)))
+            BY_TYPE(x->dtype, T, BY_MODE(stream_mode(L, x->dtype), MODE, {
+                const int threads = solo && MODE == MODE_WAVE ? 64 * (int)L.n : stream_threads(MODE);
+                EACH_LAUNCH(L, MODE == MODE_WAVE, grid, (policy_forward_kernel<T, MODE><<<solo ? 1 : grid, threads, 0, st>>>(L, p)))
+            }))
+        } else if (const int parts = split_parts(L, x->dtype)) {
+            const Split sp = {w.acc, nullptr, parts};
+            const dim3 grid((unsigned)L.n, parts);
+            BY_TYPE(x->dtype, T, BY_FLAG(p.ent != 0.0f, ENT, {
+                split_stats_kernel<T, true><<<grid, 256, 0, st>>>(L, mask, tokens, tokens_are_i64, sp);
+                policy_split_kernel<T, ENT><<<grid, 256, 0, st>>>(L, p, sp);
             }))
         } else {
             BY_TYPE(x->dtype, T, BY_FLAG(p.ent != 0.0f, ENT, {
@@ -1327,10 +1553,19 @@ extern "C" int ppo_distillation_loss(const ppo_token_logits* x, const void* teac
     if (L.n > 0) {
         count_rows(p.w, x, w, st);
         const size_t lds = teacher_lds(top);
+        const int parts = grad ? split_parts(L, x->dtype) : 0;
+        const Split sp = {w.acc, w.teach, parts};
         BY_TYPE(x->dtype, T, {
-            if (!grad)
-                EACH_LAUNCH(L, false, grid, (distill_forward_kernel<T><<<grid, stream_threads(L), lds, st>>>(L, p)))
-            else if (held_in_8(L, x->dtype))
+            if (!grad && L.n >= 512)
+                EACH_LAUNCH(L, false, grid, (distill_forward_kernel<T, MODE_BLOCK><<<grid, stream_threads(MODE_BLOCK), lds, st>>>(L, p)))
+            else if (!grad)
+                EACH_LAUNCH(L, false, grid, (distill_forward_kernel<T, MODE_FEW><<<grid, stream_threads(MODE_FEW), lds, st>>>(L, p)))
+            else if (parts) {
+                const dim3 grid((unsigned)L.n, parts);
+                split_teacher_kernel<T><<<(unsigned)L.n, 64, lds, st>>>(L, p, sp);
+                split_stats_kernel<T, false><<<grid, 256, 0, st>>>(L, mask, nullptr, 0, sp);
+                distill_split_kernel<T><<<grid, 256, lds, st>>>(L, p, sp);
+            } else if (held_in_8(L, x->dtype))
                 EACH_LAUNCH(L, false, grid, (distill_kernel<T, 8><<<grid, held_threads(L, x->dtype, 8), lds, st>>>(L, p)))
             else
                 EACH_LAUNCH(L, false, grid, (distill_kernel<T, 16><<<grid, held_threads(L, x->dtype, 16), lds, st>>>(L, p)))

@@ -210,6 +210,52 @@ def test_impossible_tokens_and_extreme_logits(dtype, v):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v,times", [(40, 1), (40, 30), (3000, 1), (20003, 20), (40001, 1), (40001, 20), (90001, 1), (140001, 18)])
+def test_losses_of_extreme_logits(v, times, dtype):
+    """Few and many rows, short and long ones, of logits so large or so low that the sums have to be taken exactly."""
+    lowest, big = torch.finfo(dtype).min, torch.finfo(dtype).max
+    x, y, _ = make(2, 1, 8, v, dtype)
+    y[:] = 17
+    x[0, 0, 3:9] = -math.inf
+    x[0, 1, 30:] = lowest
+    x[0, 2] = lowest
+    x[0, 3] = big
+    x[0, 5] = -math.inf
+    x[0, 5, 17] = 1.0
+    x[0, 6, :20] = big
+    x[0, 7] += 1000.0 if dtype != torch.float16 else 100.0
+    fx, fy, _ = flat(x, y, None)
+    lp, h = O.logprobs(fx, fy, None, 1.0)
+    old = (lp - 0.1).astype(np.float32)
+    adv = np.array([1.0, -1.0, 0.5, -0.5, 2.0, 1.0, -2.0, 1.0], np.float32)
+    w = np.full(8, 4.0 / 8)
+    loss, grad, size, _ = O.policy(fx, fy, old, adv, None, None, w, 0.2, 0.2, 0.0, 0.02, 1.0)
+    up = lambda a: torch.from_numpy(a).cuda()[None].repeat(times, 1)  # noqa: E731
+    X, Y = x.repeat(times, 1, 1), y.repeat(times, 1)
+    off = 4 * float(logp_tol(lp, v).max()) + 2.0 ** -21
+    got = K().policy_loss_and_grad(X, Y, up(old), up(adv), entropy_coef=0.02, scale=4.0 * times)
+    close(got[0], loss * times, times * mean_tol(w, (np.abs(adv) * 2 + 0.02 * (1 + h)) * off) + 2.0 ** -23 * abs(loss) * times, "loss")
+    for t in (0, times - 1):
+        close(got[2][t], lp, logp_tol(lp, v), "logprobs")
+        close(got[3][t], h, 2 * row_tol(v) * (1 + np.abs(h)) + 1e-6, "entropy")
+        close_grad(got[1][t], grad, size, v, off)
+    index = torch.tensor([17, 2, 17, v - 1], device="cuda").repeat(times, 8, 1)
+    index[:, 5, :] = 17                          # the teacher of the row with one possible token knows that one
+    index[:, 0, 1] = 1
+    index[:, 6, 3] = 1
+    index[:, 1, 3] = 5
+    values = torch.tensor([1.0, 0.5, 0.25, 0.0], device="cuda").repeat(times, 8, 1)
+    fi, ft = index[0].cpu().numpy(), f64(values[0])
+    loss, grad, size, each = O.distillation(fx, fi, ft, None, w, 1.0)
+    got = K().distillation_loss_and_grad(X, index, values, scale=4.0 * times)
+    tol = row_tol(v) + 60 * (12 * 2.0 ** -24 + 2.0 ** -22)
+    close(got[0], loss * times, times * mean_tol(w, tol + np.abs(each) * 2.0 ** -22) + 2.0 ** -23 * abs(loss) * times, "loss")
+    for t in (0, times - 1):
+        close(got[2][t], each, tol + np.abs(each) * 2.0 ** -23, "token losses")
+        close_grad(got[1][t], grad, size, v, 12 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_bad_rows_are_nan_and_leave_the_others(dtype):
     b, t, v = 1, 7, 501
     x, y, _ = make(4, b, t, v, dtype)
