@@ -355,9 +355,11 @@ typedef struct {
 size_t ppo_token_workspace_bytes(int64_t n_seq, int64_t n_tok);
 
 /* logprobs[r] of tokens[r] (int32, or int64 with tokens_are_i64) and, where entropy is not NULL, the
- * entropy of the row's distribution.  row_stats may be NULL. */
+ * entropy of the row's distribution.  row_stats may be NULL.  workspace may be NULL: a few long rows then
+ * take longer. */
 int ppo_token_logprobs(const ppo_token_logits* x, const void* tokens, int tokens_are_i64, const uint8_t* mask,
-                       float* logprobs, float* entropy, float* row_stats, void* stream);
+                       float* logprobs, float* entropy, float* row_stats, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 /* dL/dlogits from dL/dlogprob and dL/dentropy of each row (either may be NULL: zeros; each with a stride
  * for sequences and one for tokens), both times *grad_factor (device; NULL: 1).  With grad_entropy the

@@ -90,7 +90,8 @@ _SIGNATURES = {
                                      c_void_p, c_int64, c_double, c_double, c_double, c_double,
                                      c_double, c_void_p, c_void_p]),
     "ppo_token_workspace_bytes": (c_size_t, [c_int64, c_int64]),
-    "ppo_token_logprobs": (c_int, [_LOGITS_P, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "ppo_token_logprobs": (c_int, [_LOGITS_P, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                                   c_void_p]),
     "ppo_token_logprobs_backward": (c_int, [_LOGITS_P, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64,
                                             c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
     "ppo_policy_loss": (c_int, [_LOGITS_P, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p,

@@ -205,12 +205,19 @@ template <bool WAVE> __device__ __forceinline__ Part part_of() {
 // A row cut at the 16-byte boundaries of its logits: rows of an odd vocabulary begin anywhere, and reading them in
 // 16-byte steps from there was measured at 4.9 TB/s against 6.1 for aligned steps.  The logits before the first and
 // behind the last boundary, up to 7 at either end, are the edge: one scalar of threads 0-6 and 8-14.
+#define SHIFT_FROM 8192
 template <typename T> struct Span {
     int V, head, nvec;
+    int shift;                // threads before the one that takes the first vector
 
-    __device__ __forceinline__ Span(const T* x, int V) : V(V) {
+    __device__ __forceinline__ Span(const T* x, int V) : V(V), shift(0) {
         head = min(V, (int)(-(uintptr_t)x % 16u / sizeof(T)));
         nvec = (V - head) / VEC<T>;
+    }
+    // For a row whose gradient goes to `out`: the first threads stay idle so that a wave's 1 KB begins at a 128-byte line
+    // of the gradient (copying rows of 50001 bf16: 5.8 TB/s against 5.3; rows of 8 KB gain nothing).
+    __device__ __forceinline__ Span(const T* x, int V, const T* out) : Span(x, V) {
+        if (V >= SHIFT_FROM) shift = (int)((uintptr_t)(out + head) / 16u % 8u);
     }
     __device__ __forceinline__ int edge(int tid) const {      // this thread's logit of the edge, or -1
         const int behind = head + nvec * VEC<T> + tid - 8;
@@ -319,7 +326,7 @@ __device__ __forceinline__ bool stream_row(const T* x, int V, float c2, float co
 // ------------------------------------------------------------------------------------------ a row on the chip
 // A row's threads hold CH vectors each, so that statistics and gradient read memory once: 16 threads of vectors a
 // lane are 64 registers, 1024 threads then hold 256 KB.  Vectors beyond are read again for the gradient.  Vector j
-// belongs to thread j % nt; lanes past the end of the row hold its last vector, which is not counted or stored.
+// belongs to thread (j + shift) % nt; lanes beside the row hold its first or last vector, not counted and not stored.
 template <typename T, int CH> struct Row {
     u32x4 v[CH];
     float edge;
@@ -331,15 +338,16 @@ __device__ __forceinline__ void row_load(Row<T, CH>& row, const T* x, const Span
     row.edge = e >= 0 ? wide(x[e]) : -__builtin_inff();
     if (s.nvec > 0) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) row.v[i] = load_vec<false>(x + s.head, min(i * p.nt + p.tid, s.nvec - 1));
+        for (int i = 0; i < CH; ++i)
+            row.v[i] = load_vec<false>(x + s.head, max(0, min(i * p.nt + p.tid - s.shift, s.nvec - 1)));
     }
 }
 
 // A thread's part of (m, S, E), joined over the wave, in the NEAR form.
-template <typename T, int CH, bool ENT>
+template <typename T, int CH, bool WAVE, bool ENT>
 __device__ __forceinline__ Acc row_stats(Row<T, CH>& row, const T* x, const Span<T>& s, const Part& p, float c2, float counted) {
     constexpr int M = sizeof(T) == 4 ? 4 : 2;             // vectors added at once
-    const int mine = s.nvec - p.first;
+    const int mine = s.nvec + s.shift - p.first, tid = p.tid - s.shift;
     Acc a = acc_empty();
     a.n = counted;
 #pragma unroll
@@ -347,15 +355,14 @@ __device__ __forceinline__ Acc row_stats(Row<T, CH>& row, const T* x, const Span
         if (i * p.nt < mine) {
 #pragma unroll
             for (int k = i; k < i + M; ++k)
-                if (k * p.nt + 64 > mine && k * p.nt + p.tid >= s.nvec) row.v[k] = Word<T>::LOWEST;
+                if ((k * p.nt + 64 > mine && k * p.nt + tid >= s.nvec) || (k == 0 && tid < 0)) row.v[k] = Word<T>::LOWEST;
             acc_vecs<T, M, ENT, true>(a, row.v + i, c2);
         }
     }
-    if (CH == 16)
-        for (int j = CH * p.nt + p.tid; j < s.nvec; j += p.nt) {
-            const u32x4 v = load_vec<true>(x + s.head, j);
-            acc_vecs<T, 1, ENT, true>(a, &v, c2);
-        }
+    for (int j = CH * p.nt + tid; !WAVE && j < s.nvec; j += p.nt) {
+        const u32x4 v = load_vec<true>(x + s.head, j);
+        acc_vecs<T, 1, ENT, true>(a, &v, c2);
+    }
     acc_rebase<ENT, true>(a, fmaxf(a.m, row.edge), c2);
     acc_add<ENT, true>(a, row.edge, c2);
     return acc_wave<ENT, true>(a, c2);
@@ -407,24 +414,28 @@ __device__ __forceinline__ void edge_grad(const RowGrad& g, float x, T* out, int
 }
 
 // The gradient of a held row that is near.  The vectors that are read again may lie where their gradient goes.
-template <typename T, int CH, bool ENT>
+template <typename T, int CH, bool WAVE, bool ENT>
 __device__ __forceinline__ void row_grad(const Row<T, CH>& row, const T* x, T* out, const Span<T>& s, const Part& p,
                                          float c2, const RowGrad& g, bool past) {
     constexpr int N = VEC<T>;
-    const int mine = s.nvec - p.first;
+    const int mine = s.nvec + s.shift - p.first, tid = p.tid - s.shift;
     const int tok = g.tok >= 0 ? g.tok - s.head : -1;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         if (i * p.nt < mine) {
-            const int j = i * p.nt + p.tid;
+            const int j = i * p.nt + tid;
             const u32x4 o = grad_vec<T, ENT, true>(g, row.v[i], tok - j * N, c2);
-            if (j < s.nvec) store_vec(out + s.head, j, o, past);
+            if (j < s.nvec && (i > 0 || j >= 0)) store_vec(out + s.head, j, o, past);
         }
     }
-    if (CH == 16)
-        for (int j = CH * p.nt + p.tid; j < s.nvec; j += p.nt)
-            store_vec(out + s.head, j, grad_vec<T, ENT, true>(g, load_vec<false>(x + s.head, j), tok - j * N, c2), past);
+    for (int j = CH * p.nt + tid; !WAVE && j < s.nvec; j += p.nt)
+        store_vec(out + s.head, j, grad_vec<T, ENT, true>(g, load_vec<false>(x + s.head, j), tok - j * N, c2), past);
     edge_grad<T, ENT, true>(g, row.edge, out, s.edge(p.tid), c2);
+}
+
+// Vectors, and threads before them, of a piece: whole lines of the gradient.
+template <typename T> __device__ __forceinline__ int piece_of(const Span<T>& s, int segs) {
+    return ((s.nvec + s.shift + segs - 1) / segs + 7) & ~7;
 }
 
 // The gradient of a row whose statistics are known, part `seg` of `segs`; x may be out.
@@ -432,20 +443,24 @@ template <typename T, bool ENT>
 __device__ __forceinline__ void row_map(const T* x, T* out, int V, const Part& p, int seg, int segs, float c2,
                                         const RowGrad& g, bool past) {
     constexpr int N = VEC<T>;
-    const Span<T> s(x, V);
-    const int per = (s.nvec + segs - 1) / segs, end = min(s.nvec, (seg + 1) * per);
+    const Span<T> s(x, V, out);
+    const int per = piece_of(s, segs), end = min(s.nvec, (seg + 1) * per - s.shift);
     const int tok = g.tok >= 0 ? g.tok - s.head : -1;
-    for (int j = seg * per + p.tid; j < end; j += p.nt)
+    int j = seg * per + p.tid - s.shift;
+    if (j < 0) j += p.nt;
+    for (; j < end; j += p.nt)
         store_vec(out + s.head, j, grad_vec<T, ENT, false>(g, load_vec<false>(x + s.head, j), tok - j * N, c2), past);
     const int e = seg == 0 ? s.edge(p.tid) : -1;
     edge_grad<T, ENT, false>(g, e >= 0 ? wide(x[e]) : 0.0f, out, e, c2);
 }
 
 template <typename T> __device__ __forceinline__ void row_fill(T* out, int V, const Part& p, int seg, int segs, bool past) {
-    const Span<T> s(out, V);
-    const int per = (s.nvec + segs - 1) / segs, end = min(s.nvec, (seg + 1) * per);
+    const Span<T> s(out, V, out);
+    const int per = piece_of(s, segs), end = min(s.nvec, (seg + 1) * per - s.shift);
     const u32x4 zero = 0;
-    for (int j = seg * per + p.tid; j < end; j += p.nt) store_vec(out + s.head, j, zero, past);
+    int j = seg * per + p.tid - s.shift;
+    if (j < 0) j += p.nt;
+    for (; j < end; j += p.nt) store_vec(out + s.head, j, zero, past);
     const int e = seg == 0 ? s.edge(p.tid) : -1;
     if (e >= 0) out[e] = (T)0.0f;
 }
@@ -459,6 +474,7 @@ struct Logits {
     int64_t r0;               // first row of this launch
     int V;
     float c, c2;              // 1/temperature; the same times log2(e)
+    double ln2;               // c / c2
     bool past;                // the gradient is stored past the caches
 };
 
@@ -512,11 +528,11 @@ __device__ __forceinline__ float count_mask(const Weights& w, int64_t n, const P
 }
 
 __device__ __forceinline__ float row_weight(const Weights& w, const Place& at, int64_t n_tok, float counted) {
-    double d = 1.0;
-    if (w.reduction != RED_SUM && !w.mask) d = (double)w.n_seq * (double)n_tok;
-    else if (w.reduction == RED_TOKEN) d = w.count_here ? (double)counted : (double)w.totals[0];
-    else if (w.reduction == RED_SEQ) d = (double)w.seq_len[at.b] * (double)w.totals[1];
-    return (float)((double)w.scale / d);
+    float d = 1.0f;           // rows are fewer than 2^30: rounded once by 2^-24 at most, as the quotient is
+    if (w.reduction != RED_SUM && !w.mask) d = (float)(w.n_seq * n_tok);
+    else if (w.reduction == RED_TOKEN) d = w.count_here ? counted : (float)w.totals[0];
+    else if (w.reduction == RED_SEQ) d = (float)((int64_t)w.seq_len[at.b] * (int64_t)w.totals[1]);
+    return w.scale / d;
 }
 
 struct RowStats {             // what the backward pass needs of the forward pass
@@ -533,7 +549,8 @@ __device__ __forceinline__ double ln_of(float s) {
         f *= 2.0f;
         k -= 1;
     }
-    const double z = ((double)f - 1.0) / ((double)f + 1.0), y = z * z;
+    const double den = (double)f + 1.0, guess = __builtin_amdgcn_rcp(den);     // one Newton step: beyond 2^-45
+    const double z = ((double)f - 1.0) * guess * fma(-den, guess, 2.0), y = z * z;
     const double p = fma(y, fma(y, fma(y, fma(y, fma(y, 1.0 / 11, 1.0 / 9), 1.0 / 7), 1.0 / 5), 1.0 / 3), 1.0);
     return fma((double)k, LN2_D, 2.0 * z * p);
 }
@@ -542,11 +559,18 @@ __device__ __forceinline__ double ln_of(float s) {
 template <typename T> __device__ __forceinline__ float token_logit(const T* x, int64_t tok, int V) {
     return tok >= 0 && tok < V ? wide(x[tok]) : __builtin_nanf("");
 }
-__device__ __forceinline__ double logp_of(float x, float c, const Acc& a, double ln_s) {
-    return ((double)x - (double)a.m) * (double)c - ln_s;
+// ln S and ln p of a logit.  c2 is rounded: relative to 1/temperature all u_i are too long by the same factor, which
+// L.ln2 = c / c2 takes back from a single u, and, to first order, E / S from ln S.
+template <bool ENT> __device__ __forceinline__ double ln_sum(const Logits& L, const Acc& a) {
+    const double ln_s = ln_of(a.s);
+    return ENT ? fma(L.ln2 - LN2_D, (double)(a.e / a.s), ln_s) : ln_s;
 }
-__device__ __forceinline__ float entropy_of(const Acc& a, double ln_s) {
-    return (float)(ln_s - LN2_D * (double)(a.e / a.s));
+template <bool NEAR> __device__ __forceinline__ double logp_of(const Logits& L, float x, float m, double ln_s) {
+    const double u = NEAR ? fma((double)x, (double)L.c2, -(double)near_max(m, L.c2)) : ((double)x - (double)m) * (double)L.c2;
+    return fma(L.ln2, u, -ln_s);
+}
+__device__ __forceinline__ float entropy_of(const Logits& L, const Acc& a, double ln_s) {
+    return (float)fma(-L.ln2, (double)(a.e / a.s), ln_s);
 }
 
 // ------------------------------------------------------------------------------------------ counting masks
@@ -623,11 +647,11 @@ __global__ __launch_bounds__(1024, 4) void logprobs_kernel(Logits L, const void*
         const float xt = token_logit(x, int_at(tokens, i64, r), L.V);
         Acc a;
         if (!stream_row<T, MODE, ENT, KEEP>(x, L.V, L.c2, 0.0f, lds, a)) return;
-        const double ln_s = ln_of(a.s);
-        lp = logp_of(xt, L.c, a, ln_s);
+        const double ln_s = ln_sum<ENT>(L, a);
+        lp = logp_of<false>(L, xt, a.m, ln_s);
         st.m = a.m;
         st.s = a.s;
-        if (ENT) st.h = entropy_of(a, ln_s);
+        if (ENT) st.h = entropy_of(L, a, ln_s);
     }
     if (part_of<WAVE>().tid == 0) {
         if (logprobs) logprobs[r] = (float)lp;
@@ -637,15 +661,16 @@ __global__ __launch_bounds__(1024, 4) void logprobs_kernel(Logits L, const void*
     }
 }
 
-__device__ __forceinline__ RowGrad grad_seed(float m, float s, float h, float g_lp, float g_h, int64_t tok, int V,
-                                             float c) {
+// h, ln_s: of a form's statistics; used with an entropy gradient only
+__device__ __forceinline__ RowGrad grad_seed(const Logits& L, float m, float s, float h, float ln_s, float g_lp, float g_h,
+                                             int64_t tok) {
     RowGrad g;
     g.m = m;
-    const float ln_s = (float)ln_of(s);
-    const bool bad = tok < 0 || tok >= V;
-    g.a = bad ? __builtin_nanf("") : -c * (g_lp + g_h * (h - ln_s)) / s;
-    g.b = -c * g_h * (float)LN2_D / s;
-    g.gt = c * g_lp;
+    const bool bad = tok < 0 || tok >= L.V;
+    const float k = -L.c / s;
+    g.a = bad ? __builtin_nanf("") : k * fmaf(g_h, h - ln_s, g_lp);
+    g.b = k * g_h * (float)L.ln2;
+    g.gt = L.c * g_lp;
     g.tok = bad ? -1 : (int)tok;
     return g;
 }
@@ -657,7 +682,7 @@ struct Incoming {             // dL/dlogp and dL/dH of each row, and a factor on
 
 // Rows in the reverse of the forward pass's order: what it read last is still in the 256 MB cache in front of the HBM.
 template <typename T, bool WAVE, bool ENT>
-__global__ __launch_bounds__(256) void backward_kernel(Logits L, const void* tokens, int i64, const uint8_t* mask,
+__global__ __launch_bounds__(1024) void backward_kernel(Logits L, const void* tokens, int i64, const uint8_t* mask,
                                                        const RowStats* __restrict__ stats, Incoming in) {
     const int64_t r = L.n - 1 - row_of<WAVE>(L);
     if (WAVE && r < 0) return;
@@ -672,7 +697,7 @@ __global__ __launch_bounds__(256) void backward_kernel(Logits L, const void* tok
     const RowStats st = stats[r];
     const float g_lp = in.lp ? f * in.lp[at.b * in.lp_s + at.t * in.lp_t] : 0.0f;
     const float g_h = ENT ? f * in.h[at.b * in.h_s + at.t * in.h_t] : 0.0f;
-    const RowGrad g = grad_seed(st.m, st.s, st.h, g_lp, g_h, int_at(tokens, i64, r), L.V, L.c);
+    const RowGrad g = grad_seed(L, st.m, st.s, st.h, ENT ? (float)ln_of(st.s) : 0.0f, g_lp, g_h, int_at(tokens, i64, r));
     row_map<T, ENT>(row_in<T>(L, at), out, L.V, p, blockIdx.y, gridDim.y, L.c2, g, L.past);
 }
 
@@ -691,32 +716,42 @@ struct PolicyArgs {
     float* solo;              // the loss, where one workgroup has all rows
 };
 
+// Gradients of a counted row's loss, and the parts that the loss itself is made of afterwards.
 struct PolicyRow {
-    double loss;              // weighted, as the gradients are
-    float g_lp, g_h;
+    float g_lp, g_h, w, kl;
+    double surrogate;
 };
 
-__device__ __forceinline__ PolicyRow policy_row(const PolicyArgs& p, double lp, float h, float old_lp, float adv,
-                                                float ref, float w) {
+__device__ __forceinline__ PolicyRow policy_row(const PolicyArgs& p, double lp, float old_lp, float adv, float ref, float w) {
     // Differences of log-probabilities are formed in fp64, where they lose nothing.  The ratio is 1 + (e^d - 1) with
     // the second part in fp32: near 1 that keeps more of it than fp32 does, and a loss is a mean in which A and -A
     // nearly cancel.
+    PolicyRow o;
     const double r = 1.0 + (double)expm1f((float)(lp - (double)old_lp)), a = (double)adv;
     const bool clipped = (adv > 0.0f && r > (double)p.hi) || (adv < 0.0f && r < (double)p.lo);
-    double loss = clipped ? -(adv > 0.0f ? (double)p.hi : (double)p.lo) * a : -r * a;
+    o.surrogate = clipped ? (adv > 0.0f ? (double)p.hi : (double)p.lo) * a : r * a;
     float g = clipped ? 0.0f : (float)(-r * a);
+    o.kl = 0.0f;
     if (p.kl != 0.0f) {
         const float d = (float)((double)ref - lp);
         // e^d - 1 - d: its series where the difference would cancel (|d|^6 / 20160 < 2^-24 at 1/4)
         const float em1 = expm1f(d);
-        const float k = fabsf(d) < 0.25f
+        o.kl = fabsf(d) < 0.25f
             ? d * d * fmaf(d, fmaf(d, fmaf(d, fmaf(d, fmaf(d, 1.0f / 5040, 1.0f / 720), 1.0f / 120), 1.0f / 24), 1.0f / 6), 0.5f)
             : em1 - d;
-        loss = fma((double)p.kl, (double)k, loss);
         g = fmaf(-p.kl, em1, g);
     }
+    o.g_lp = w * g;
+    o.g_h = -w * p.ent;
+    o.w = w;
+    return o;
+}
+
+__device__ __forceinline__ double weighted_loss(const PolicyArgs& p, const PolicyRow& o, float h) {
+    double loss = -o.surrogate;
+    if (p.kl != 0.0f) loss = fma((double)p.kl, (double)o.kl, loss);
     if (p.ent != 0.0f) loss = fma(-(double)p.ent, (double)h, loss);
-    return {loss * (double)w, w * g, -w * p.ent};
+    return o.w != 0.0f ? loss * (double)o.w : 0.0;      // a row that does not count
 }
 
 // inputs of a counted row
@@ -760,14 +795,18 @@ struct PolicyDone {
     float h;
     PolicyRow o;
 };
+template <bool NEAR>
 __device__ __forceinline__ PolicyDone policy_done(const Logits& L, const PolicyArgs& p, const PolicyIn& in, const Acc& a,
                                                   const Place& at, float counted) {
     PolicyDone d;
-    d.ln_s = ln_of(a.s);
-    d.lp = logp_of(in.xt, L.c, a, d.ln_s);
-    d.h = entropy_of(a, d.ln_s);
-    d.o = policy_row(p, d.lp, d.h, in.old_lp, in.adv, in.ref, row_weight(p.w, at, L.n_tok, counted));
+    d.ln_s = ln_sum<true>(L, a);
+    d.lp = logp_of<NEAR>(L, in.xt, a.m, d.ln_s);
+    d.h = entropy_of(L, a, d.ln_s);
+    d.o = policy_row(p, d.lp, in.old_lp, in.adv, in.ref, row_weight(p.w, at, L.n_tok, counted));
     return d;
+}
+__device__ __forceinline__ RowGrad policy_seed(const Logits& L, const PolicyDone& d, float m, float s, int64_t tok) {
+    return grad_seed(L, m, s, d.h, (float)d.ln_s, d.o.g_lp, d.o.g_h, tok);
 }
 
 // Forward only; leaves what the backward pass needs.
@@ -776,7 +815,7 @@ __global__ __launch_bounds__(1024, 4) void policy_forward_kernel(Logits L, Polic
     constexpr bool WAVE = MODE == MODE_WAVE;
     __shared__ Acc lds[16];
     const int64_t r = row_of<WAVE>(L);
-    PolicyDone d = {0.0, 0.0, 0.0f, {0.0, 0.0f, 0.0f}};
+    PolicyDone d = {};
     if (!WAVE || r < L.n) {
         RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
         if (!p.w.mask || p.w.mask[r]) {
@@ -785,7 +824,7 @@ __global__ __launch_bounds__(1024, 4) void policy_forward_kernel(Logits L, Polic
             const PolicyIn in = policy_in(L, p, x, r, at);
             Acc a;
             if (!stream_row<T, MODE, true, true>(x, L.V, L.c2, count_mask(p.w, L.n, part_of<WAVE>()), lds, a)) return;
-            d = policy_done(L, p, in, a, at, a.n);
+            d = policy_done<false>(L, p, in, a, at, a.n);
             st = {a.m, a.s, d.h, 0.0f};
         }
         if (part_of<WAVE>().tid == 0) {
@@ -798,7 +837,7 @@ __global__ __launch_bounds__(1024, 4) void policy_forward_kernel(Logits L, Polic
             }
         }
     }
-    row_loss<WAVE>(p, r, L.n, d.o.loss);
+    row_loss<WAVE>(p, r, L.n, weighted_loss(p, d.o, d.h));
 }
 
 // Loss and gradient: the row stays on the chip between its statistics and its gradient.  The first wave makes of the
@@ -814,19 +853,19 @@ __global__ __launch_bounds__(1024, 4) void policy_kernel(Logits L, PolicyArgs p)
     __shared__ RowShared sh;
     const Part q = part_of<WAVE>();
     const int64_t r = row_of<WAVE>(L);
-    PolicyDone d = {0.0, 0.0, 0.0f, {0.0, 0.0f, 0.0f}};
+    PolicyDone d = {};
     if (!WAVE || r < L.n) {
         const Place at = place_of(L, r);
         T* out = row_out<T>(L, at);
         if (!p.w.mask || p.w.mask[r]) {
             const T* x = row_in<T>(L, at);
-            const Span<T> s(x, L.V);
+            const Span<T> s = WAVE ? Span<T>(x, L.V) : Span<T>(x, L.V, out);
             Row<T, CH> row;
             const PolicyIn in = policy_in(L, p, x, r, at);
             row_load(row, x, s, q);
             const float counted = count_mask(p.w, L.n, q);
             asm volatile("" :: "v"(in.xt));   // read before the barrier: the gradient may overwrite it
-            Acc a = row_stats<T, CH, true>(row, x, s, q, L.c2, counted);
+            Acc a = row_stats<T, CH, WAVE, true>(row, x, s, q, L.c2, counted);
             RowGrad g;
             bool near_ = true;
             if (!WAVE) {
@@ -836,8 +875,8 @@ __global__ __launch_bounds__(1024, 4) void policy_kernel(Logits L, PolicyArgs p)
             if (WAVE || q.first == 0) {
                 if (!WAVE) a = acc_waves<true, true>(sh.acc, L.c2);
                 near_ = is_near(a.m, L.c2);
-                d = policy_done(L, p, in, near_done(a, L.c2), at, a.n);
-                g = grad_seed(near_max(a.m, L.c2), a.s, d.h, d.o.g_lp, d.o.g_h, in.tok, L.V, L.c);
+                d = policy_done<true>(L, p, in, a, at, a.n);
+                g = policy_seed(L, d, near_max(a.m, L.c2), a.s, in.tok);
                 if (!WAVE && threadIdx.x == 0) {
                     sh.grad = g;
                     sh.near_ = near_;
@@ -849,17 +888,17 @@ __global__ __launch_bounds__(1024, 4) void policy_kernel(Logits L, PolicyArgs p)
                 near_ = sh.near_;
             }
             if (near_) {
-                row_grad<T, CH, ENT_GRAD>(row, x, out, s, q, L.c2, g, L.past);
+                row_grad<T, CH, WAVE, ENT_GRAD>(row, x, out, s, q, L.c2, g, L.past);
             } else {
                 const float n = a.n;
                 a = far_stats<T, WAVE, true>(x, s, q, L.c2, sh.acc);
-                d = policy_done(L, p, in, a, at, n);      // (n: the first wave's, which alone uses the weighted results)
+                d = policy_done<false>(L, p, in, a, at, n);      // (n: the first wave's, which alone uses the weighted results)
                 if (!WAVE) {
-                    if (threadIdx.x == 0) sh.grad = grad_seed(a.m, a.s, d.h, d.o.g_lp, d.o.g_h, in.tok, L.V, L.c);
+                    if (threadIdx.x == 0) sh.grad = policy_seed(L, d, a.m, a.s, in.tok);
                     __syncthreads();
                     g = sh.grad;
                 } else {
-                    g = grad_seed(a.m, a.s, d.h, d.o.g_lp, d.o.g_h, in.tok, L.V, L.c);
+                    g = policy_seed(L, d, a.m, a.s, in.tok);
                 }
                 row_map<T, ENT_GRAD>(x, out, L.V, q, 0, 1, L.c2, g, L.past);
             }
@@ -871,7 +910,7 @@ __global__ __launch_bounds__(1024, 4) void policy_kernel(Logits L, PolicyArgs p)
             if (p.entropy) p.entropy[r] = d.h;
         }
     }
-    row_loss<WAVE>(p, r, L.n, d.o.loss);
+    row_loss<WAVE>(p, r, L.n, weighted_loss(p, d.o, d.h));
 }
 
 // Few long rows: a row in `parts` pieces of a workgroup each, first their statistics (split_stats_kernel), then, in a
@@ -884,6 +923,7 @@ struct Split {
     int parts;
 };
 
+// blockIdx.y: the piece
 template <typename T, bool ENT>
 __global__ __launch_bounds__(256) void split_stats_kernel(Logits L, const uint8_t* mask, const void* tokens, int i64, Split sp) {
     __shared__ Acc lds[16];
@@ -906,6 +946,27 @@ template <bool ENT> __device__ __forceinline__ Acc split_join(const Split& sp, i
     return acc_wave<ENT>(a, c2);
 }
 
+// Log-probabilities of rows that were cut, a wave each.
+template <bool ENT>
+__global__ __launch_bounds__(256) void split_logprobs_kernel(Logits L, const uint8_t* mask, float* logprobs, double* logprobs64,
+                                                             float* entropy, RowStats* stats, Split sp) {
+    const int64_t r = row_of<true>(L);
+    if (r >= L.n) return;
+    double lp = 0.0;
+    RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
+    if (!mask || mask[r]) {
+        const Acc a = split_join<ENT>(sp, r, L.c2);
+        const double ln_s = ln_sum<ENT>(L, a);
+        lp = logp_of<false>(L, sp.acc[r * sp.parts].n, a.m, ln_s);
+        st = {a.m, a.s, ENT ? entropy_of(L, a, ln_s) : 0.0f, 0.0f};
+    }
+    if ((threadIdx.x & 63) > 0) return;
+    if (logprobs) logprobs[r] = (float)lp;
+    if (logprobs64) logprobs64[r] = lp;
+    if (ENT && entropy) entropy[r] = st.h;
+    if (stats) stats[r] = st;
+}
+
 template <typename T, bool ENT_GRAD>
 __global__ __launch_bounds__(256) void policy_split_kernel(Logits L, PolicyArgs p, Split sp) {
     __shared__ RowShared sh;
@@ -913,7 +974,7 @@ __global__ __launch_bounds__(256) void policy_split_kernel(Logits L, PolicyArgs 
     const int64_t r = blockIdx.x;
     const Place at = place_of(L, r);
     T* out = row_out<T>(L, at);
-    PolicyDone d = {0.0, 0.0, 0.0f, {0.0, 0.0f, 0.0f}};
+    PolicyDone d = {};
     if (!p.w.mask || p.w.mask[r]) {
         if (q.first == 0) {
             PolicyIn in;
@@ -923,8 +984,8 @@ __global__ __launch_bounds__(256) void policy_split_kernel(Logits L, PolicyArgs 
             in.ref = p.ref ? p.ref[r] : 0.0f;
             in.xt = sp.acc[r * sp.parts].n;
             const Acc a = split_join<true>(sp, r, L.c2);
-            d = policy_done(L, p, in, a, at, wave_sum(count_mask(p.w, L.n, part_of<true>())));
-            if (threadIdx.x == 0) sh.grad = grad_seed(a.m, a.s, d.h, d.o.g_lp, d.o.g_h, in.tok, L.V, L.c);
+            d = policy_done<false>(L, p, in, a, at, wave_sum(count_mask(p.w, L.n, part_of<true>())));
+            if (threadIdx.x == 0) sh.grad = policy_seed(L, d, a.m, a.s, in.tok);
         }
         __syncthreads();
         row_map<T, ENT_GRAD>(row_in<T>(L, at), out, L.V, q, blockIdx.y, gridDim.y, L.c2, sh.grad, L.past);
@@ -936,7 +997,7 @@ __global__ __launch_bounds__(256) void policy_split_kernel(Logits L, PolicyArgs 
         p.logprobs[r] = (float)d.lp;
         if (p.entropy) p.entropy[r] = d.h;
     }
-    row_loss<false>(p, r, L.n, d.o.loss);
+    row_loss<false>(p, r, L.n, weighted_loss(p, d.o, d.h));
 }
 
 // ------------------------------------------------------------------------------------------ preference loss
@@ -1037,11 +1098,11 @@ __device__ __forceinline__ float teacher_load(const TeacherArgs& p, const Logits
 }
 
 // First wave only: sum q (ln q - ln p).
-__device__ __forceinline__ float teacher_loss(const TeacherArgs& p, const Teacher& s, float ent, const Acc& a, float c) {
-    const double ln_s = ln_of(a.s);
+__device__ __forceinline__ float teacher_loss(const TeacherArgs& p, const Teacher& s, float ent, const Acc& a, const Logits& L) {
+    const double ln_s = ln_sum<false>(L, a);
     double cross = 0.0;
     for (int k = threadIdx.x; k < p.K; k += 64)
-        if (s.q[k] != 0.0f) cross += (double)s.q[k] * logp_of(s.x[k], c, a, ln_s);
+        if (s.q[k] != 0.0f) cross += (double)s.q[k] * logp_of<false>(L, s.x[k], a.m, ln_s);
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) cross += __shfl_xor(cross, off);
     return *s.bad ? __builtin_nanf("") : (float)((double)ent - cross);
@@ -1058,13 +1119,13 @@ __device__ __forceinline__ void teacher_places(const TeacherArgs& p, const Teach
                                                const RowGrad& rg, float g, const Span<T>& w, int seg = 0, int segs = 1) {
     __syncthreads();          // the bulk is written
     if (*s.bad) return;
-    const int per = (w.nvec + segs - 1) / segs;
+    const int per = piece_of(w, segs);
     for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
         const int i = s.index[k];
         if (i < 0) continue;
         if (segs > 1) {       // of this piece only; the edge is the first one's
             const int j = i < w.head ? -1 : (i - w.head) / VEC<T>;
-            if ((j < 0 || j >= w.nvec ? 0 : j / per) != seg) continue;
+            if ((j < 0 || j >= w.nvec ? 0 : (j + w.shift) / per) != seg) continue;
         }
         float all = 0.0f;     // a token that appears twice: both entries, in both places the same number
         for (int j = 0; j < p.K; ++j) all += s.index[j] == i ? s.q[j] : 0.0f;
@@ -1087,7 +1148,7 @@ __global__ __launch_bounds__(1024, 4) void distill_forward_kernel(Logits L, Teac
         if (threadIdx.x < 64) ent = teacher_load(p, L, r, x, teach);
         Acc a;
         if (!stream_row<T, MODE, false, true>(x, L.V, L.c2, count_mask(p.w, L.n, part_of<false>()), lds, a)) return;
-        loss = teacher_loss(p, teach, ent, a, L.c) / (L.c * L.c);
+        loss = teacher_loss(p, teach, ent, a, L) / (L.c * L.c);
         st.m = a.m;
         st.s = a.s;
         st.w = row_weight(p.w, at, L.n_tok, a.n);
@@ -1112,12 +1173,12 @@ __global__ __launch_bounds__(1024, 4) void distill_kernel(Logits L, TeacherArgs 
     float loss = 0.0f, w = 0.0f;
     if (!p.w.mask || p.w.mask[r]) {
         const T* x = row_in<T>(L, at);
-        const Span<T> s(x, L.V);
+        const Span<T> s(x, L.V, out);
         Row<T, CH> row;
         row_load(row, x, s, q);
         float ent = 0.0f;
         if (q.first == 0) ent = teacher_load(p, L, r, x, teach);
-        Acc a = row_stats<T, CH, false>(row, x, s, q, L.c2, count_mask(p.w, L.n, q));
+        Acc a = row_stats<T, CH, false, false>(row, x, s, q, L.c2, count_mask(p.w, L.n, q));
         if ((threadIdx.x & 63) == 0) sh.acc[threadIdx.x >> 6] = a;
         __syncthreads();
         a = acc_waves<false, true>(sh.acc, L.c2);
@@ -1125,7 +1186,7 @@ __global__ __launch_bounds__(1024, 4) void distill_kernel(Logits L, TeacherArgs 
         const float scale = w / L.c;
         if (is_near(a.m, L.c2)) {
             const RowGrad g = teacher_seed(teach, near_max(a.m, L.c2), a.s, scale);
-            row_grad<T, CH, false>(row, x, out, s, q, L.c2, g, L.past);
+            row_grad<T, CH, false, false>(row, x, out, s, q, L.c2, g, L.past);
             teacher_places<T, true>(p, teach, out, L, g, scale, s);
             a = near_done(a, L.c2);
         } else {
@@ -1135,7 +1196,7 @@ __global__ __launch_bounds__(1024, 4) void distill_kernel(Logits L, TeacherArgs 
             row_map<T, false>(x, out, L.V, q, 0, 1, L.c2, g, L.past);
             teacher_places<T, false>(p, teach, out, L, g, scale, s);
         }
-        if (q.first == 0) loss = teacher_loss(p, teach, ent, a, L.c) / (L.c * L.c);
+        if (q.first == 0) loss = teacher_loss(p, teach, ent, a, L) / (L.c * L.c);
     } else {
         row_fill(out, L.V, q, 0, 1, L.past);
     }
@@ -1146,17 +1207,26 @@ __global__ __launch_bounds__(1024, 4) void distill_kernel(Logits L, TeacherArgs 
     }
 }
 
-// Few long rows, as policy_split_kernel: the teacher's entries are made by a workgroup of their own beside the pieces'
-// statistics, because another piece's gradient may lie where the policy's logits of the entries were.
-template <typename T> __global__ __launch_bounds__(64) void split_teacher_kernel(Logits L, TeacherArgs p, Split sp) {
+// Few long rows, as policy_split_kernel.  A workgroup beside the pieces' makes the teacher's entries, because another
+// piece's gradient may lie where the policy's logits of the entries were.
+template <typename T> __global__ __launch_bounds__(256) void split_teacher_kernel(Logits L, TeacherArgs p, Split sp) {
+    __shared__ Acc lds[16];
     extern __shared__ int entries[];
-    const Teacher teach(entries, p.K);
     const int64_t r = blockIdx.x;
     if (p.w.mask && !p.w.mask[r]) return;
-    const float ent = teacher_load(p, L, r, row_in<T>(L, place_of(L, r)), teach);
+    const T* x = row_in<T>(L, place_of(L, r));
+    if ((int)blockIdx.y < sp.parts) {
+        Acc a;
+        if (!stream_row<T, MODE_BLOCK, false, true>(x, L.V, L.c2, 0.0f, lds, a, blockIdx.y, sp.parts)) return;
+        if (threadIdx.x == 0) sp.acc[r * sp.parts + blockIdx.y] = a;
+        return;
+    }
+    const Teacher teach(entries, p.K);
+    float ent = 0.0f;
+    if (threadIdx.x < 64) ent = teacher_load(p, L, r, x, teach);
     __syncthreads();
     int* to = sp.teach + r * TEACHER_WORDS;
-    for (int k = threadIdx.x; k < 2 + 3 * p.K; k += 64) to[k < 2 ? k : k + 2] = entries[k];
+    for (int k = threadIdx.x; k < 2 + 3 * p.K; k += 256) to[k < 2 ? k : k + 2] = entries[k];
     if (threadIdx.x == 0) to[2] = __float_as_int(ent);
 }
 
@@ -1183,8 +1253,8 @@ template <typename T> __global__ __launch_bounds__(256) void distill_split_kerne
         const T* x = row_in<T>(L, at);
         const RowGrad g = teacher_seed(teach, a.m, a.s, w / L.c);
         row_map<T, false>(x, out, L.V, q, blockIdx.y, gridDim.y, L.c2, g, L.past);
-        teacher_places<T, false>(p, teach, out, L, g, w / L.c, Span<T>(x, L.V), blockIdx.y, gridDim.y);
-        if (q.first == 0) loss = teacher_loss(p, teach, __int_as_float(from[2]), a, L.c) / (L.c * L.c);
+        teacher_places<T, false>(p, teach, out, L, g, w / L.c, Span<T>(x, L.V, out), blockIdx.y, gridDim.y);
+        if (q.first == 0) loss = teacher_loss(p, teach, __int_as_float(from[2]), a, L) / (L.c * L.c);
     } else {
         row_fill(out, L.V, q, blockIdx.y, gridDim.y, L.past);
     }
@@ -1194,7 +1264,7 @@ template <typename T> __global__ __launch_bounds__(256) void distill_split_kerne
     else p.part[r] = (double)w * (double)loss;
 }
 
-template <typename T> __global__ __launch_bounds__(256) void distill_backward_kernel(Logits L, TeacherArgs p) {
+template <typename T> __global__ __launch_bounds__(1024) void distill_backward_kernel(Logits L, TeacherArgs p) {
     extern __shared__ int entries[];
     const Teacher teach(entries, p.K);
     const int64_t r = L.n - 1 - row_of<false>(L);   // as in backward_kernel
@@ -1212,14 +1282,14 @@ template <typename T> __global__ __launch_bounds__(256) void distill_backward_ke
     const float g = (p.factor ? *p.factor : 1.0f) * st.w / L.c;
     const RowGrad rg = teacher_seed(teach, st.m, st.s, g);
     row_map<T, false>(x, out, L.V, q, 0, 1, L.c2, rg, L.past);
-    teacher_places<T, false>(p, teach, out, L, rg, g, Span<T>(x, L.V));
+    teacher_places<T, false>(p, teach, out, L, rg, g, Span<T>(x, L.V, out));
 }
 
 // ------------------------------------------------------------------------------------------ host side
 #define ALIGN256(n) (((size_t)(n) + 255) & ~(size_t)255)
 
 #define TOTAL_GRID 64
-#define SPLIT_ROWS 128
+#define SPLIT_ROWS 128        // rows that are ever cut
 
 struct Workspace {            // one call's scratch
     double *part, *sums;      // weighted loss of each row (or pair); TOTAL_GRID sums of them
@@ -1245,7 +1315,7 @@ static Workspace carve(void* base, int64_t n_seq, int64_t n_tok) {
     w.stats = (RowStats*)take(sizeof(RowStats) * (size_t)(n_seq * n_tok));
     const size_t few = (size_t)(n_seq * n_tok < SPLIT_ROWS ? n_seq * n_tok : SPLIT_ROWS);
     w.acc = (Acc*)take(sizeof(Acc) * few * SPLIT_PARTS);
-    w.teach = (int*)take(4 * few * TEACHER_WORDS);
+    w.teach = (int*)take(4 * (few < 64 ? few : 64) * TEACHER_WORDS);
     w.bytes = (size_t)(p - (char*)base);
     return w;
 }
@@ -1286,6 +1356,7 @@ static Logits logits_of(const ppo_token_logits* x, void* grad) {
     L.V = (int)x->vocab;
     L.c = x->inv_temperature;
     L.c2 = x->inv_temperature * LOG2E_F;
+    L.ln2 = (double)L.c / (double)L.c2;
     // A gradient that the 256 MB cache cannot hold is stored past it: 32768 bf16 logits a row, loss and gradient and a
     // copy of the gradient after it take 200 us against 208 at 256 MB, but 99 against 81 at 128 MB.
     L.past = L.n * L.V * (x->dtype == PPO_F32 ? 4 : 2) > (int64_t)192 << 20;
@@ -1326,21 +1397,26 @@ static int stream_threads(int mode) { return mode == MODE_FEW ? 1024 : 256; }
     else if ((mode) == MODE_BLOCK) { constexpr int M = MODE_BLOCK; __VA_ARGS__; }  \
     else { constexpr int M = MODE_FEW; __VA_ARGS__; }
 
-// Pieces of a row where there are so few long ones that they leave most of the chip idle; 0: the row is not cut.
-static int split_parts(const Logits& L, int dtype) {
-    if (L.n > SPLIT_ROWS || row_bytes(L, dtype) < 65536) return 0;
+// Pieces of a row where there are so few long ones (at most `rows`, of `bytes` at least) that they leave most of the chip
+// idle; 0: the row is not cut.  Device time of bf16 rows of 256 KB, whole / cut: policy loss with gradient 1 row 20 / 7.4 us,
+// 16 rows 22 / 10, 128 rows 29 / 24 (rows of 32 KB: 6.6 / 7); distillation 1 row
+// 20 / 10, 64 rows 26 / 19, 128 rows 29 / 32; log-probabilities 1 row 11 / 5.5, 64 rows 12 / 9, 256 rows 17 / 17.
+static int split_parts(const Logits& L, int dtype, int64_t rows, int64_t bytes) {
+    if (L.n > rows || row_bytes(L, dtype) < bytes) return 0;
     const int64_t most = row_bytes(L, dtype) / 8192, want = 1024 / L.n;
     const int64_t parts = want < most ? want : most;
     return (int)(parts < SPLIT_PARTS ? parts : SPLIT_PARTS);
 }
 
-// Threads of a row that is held in CH vectors each: as many as it needs.
+// Threads of a row that is held in CH vectors each: as many as it needs (a shift may leave up to 7
+// vectors over, which are read twice).
 static int held_threads(const Logits& L, int dtype, int CH) {
     const int64_t waves = (row_bytes(L, dtype) + (int64_t)CH * 16 * 64 - 1) / ((int64_t)CH * 16 * 64);
     return (int)(waves < 16 ? waves : 16) * 64;
 }
-// 8 vectors where 1024 threads hold the row so, else 16 (and the rest of a row beyond 256 KB is read twice)
-static bool held_in_8(const Logits& L, int dtype) { return row_bytes(L, dtype) <= 8 * 16 * 1024; }
+// 8 vectors a thread for rows of up to 96 KB, else 16 (4096 rows with their gradient: of 80 KB 122 us against 131 with 16,
+// of 100 KB 187 against 161); the rest of a row beyond 256 KB is read twice.
+static bool held_in_8(const Logits& L, int dtype) { return row_bytes(L, dtype) <= 96 * 1024; }
 
 static void launch_total(const Workspace& w, int64_t n, float* loss, hipStream_t st) {
     if (n <= 16384) {
@@ -1373,35 +1449,50 @@ static int weights_of(Weights* o, const uint8_t* mask, int reduction, float scal
 }
 
 static void launch_logprobs(Logits L, int dtype, const void* tokens, int i64, const uint8_t* mask, float* logprobs,
-                            double* logprobs64, float* entropy, RowStats* stats, hipStream_t st) {
+                            double* logprobs64, float* entropy, RowStats* stats, Acc* acc, hipStream_t st) {
+    if (const int parts = acc ? split_parts(L, dtype, 64, 128 * 1024) : 0) {
+        const Split sp = {acc, nullptr, parts};
+        BY_FLAG(entropy != nullptr, ENT, {
+            BY_TYPE(dtype, T, (split_stats_kernel<T, ENT><<<dim3((unsigned)L.n, parts), 256, 0, st>>>(L, mask, tokens, i64, sp)))
+            split_logprobs_kernel<ENT><<<(int)(L.n + 3) / 4, 256, 0, st>>>(L, mask, logprobs, logprobs64, entropy, stats, sp);
+        })
+        return;
+    }
     BY_TYPE(dtype, T, BY_MODE(stream_mode(L, dtype), MODE, BY_FLAG(entropy != nullptr, ENT, BY_FLAG(stats != nullptr, KEEP, {
         EACH_LAUNCH(L, MODE == MODE_WAVE, grid, (logprobs_kernel<T, MODE, ENT, KEEP><<<grid, stream_threads(MODE), 0, st>>>(
             L, tokens, i64, mask, logprobs, logprobs64, entropy, stats)))
     }))))
 }
 
-// Parts of a row that the backward pass gives to a workgroup each, so that few rows fill the chip too: at least 16 KB.
+// Threads of a row in the backward pass: 1024 of long rows (rows of 64 KB: 127 us against 134 with 256), 256 of rows that
+// would leave them without work (rows of 8 KB: 83 us against 128).
+static int backward_threads(const Logits& L, int dtype) { return row_bytes(L, dtype) >= 32768 ? 1024 : 256; }
+
+// Parts of a row that the backward pass gives to a workgroup each, so that few rows fill the chip too: at least 64 KB.
 static int backward_parts(const Logits& L, int dtype) {
-    const int64_t want = (1024 + L.n - 1) / L.n, most = (row_bytes(L, dtype) + 16383) / 16384;
+    const int64_t want = (1024 + L.n - 1) / L.n, most = (row_bytes(L, dtype) + 65535) / 65536;
     return (int)(want < most ? want : most);
 }
 
 extern "C" int ppo_token_logprobs(const ppo_token_logits* x, const void* tokens, int tokens_are_i64,
-                                  const uint8_t* mask, float* logprobs, float* entropy, float* row_stats, void* stream) {
+                                  const uint8_t* mask, float* logprobs, float* entropy, float* row_stats, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
     const int e = check_logits(x, nullptr);
     if (e) return e;
     Logits L = logits_of(x, nullptr);
     if (L.n == 0) return 0;
     if (!tokens || !logprobs) return PPO_E_BADARG;
+    const Workspace w = carve(workspace, x->n_seq, x->n_tok);
+    if (workspace && workspace_bytes < w.bytes) return PPO_E_WORKSPACE;
     launch_logprobs(L, x->dtype, tokens, tokens_are_i64, mask, logprobs, nullptr, entropy, (RowStats*)row_stats,
-                    (hipStream_t)stream);
+                    workspace ? w.acc : nullptr, (hipStream_t)stream);
     return (int)hipGetLastError();
 }
 
 static int launch_backward(Logits L, int dtype, const void* tokens, int i64, const uint8_t* mask,
                            const RowStats* stats, const Incoming& in, hipStream_t st) {
     BY_TYPE(dtype, T, BY_FLAG(by_wave(L, dtype), WAVE, BY_FLAG(in.h != nullptr, ENT, {
-        EACH_LAUNCH(L, WAVE, grid, (backward_kernel<T, WAVE, ENT><<<dim3(grid, WAVE ? 1 : backward_parts(L, dtype)), 256, 0, st>>>(
+        EACH_LAUNCH(L, WAVE, grid, (backward_kernel<T, WAVE, ENT><<<dim3(grid, WAVE ? 1 : backward_parts(L, dtype)), WAVE ? 256 : backward_threads(L, dtype), 0, st>>>(
             L, tokens, i64, mask, stats, in)))
     })))
     return (int)hipGetLastError();
@@ -1466,7 +1557,7 @@ extern "C" int ppo_policy_loss(const ppo_token_logits* x, const void* tokens, in
                 const int threads = solo && MODE == MODE_WAVE ? 64 * (int)L.n : stream_threads(MODE);
                 EACH_LAUNCH(L, MODE == MODE_WAVE, grid, (policy_forward_kernel<T, MODE><<<solo ? 1 : grid, threads, 0, st>>>(L, p)))
             }))
-        } else if (const int parts = split_parts(L, x->dtype)) {
+        } else if (const int parts = split_parts(L, x->dtype, 128, 64 * 1024)) {
             const Split sp = {w.acc, nullptr, parts};
             const dim3 grid((unsigned)L.n, parts);
             BY_TYPE(x->dtype, T, BY_FLAG(p.ent != 0.0f, ENT, {
@@ -1504,7 +1595,7 @@ extern "C" int ppo_preference_loss(const ppo_token_logits* x, const void* tokens
     RowStats* stats = row_stats ? (RowStats*)row_stats : w.stats;
     float* sd = seeds ? seeds : w.seeds;
     if (L.n > 0) {
-        launch_logprobs(L, x->dtype, tokens, tokens_are_i64, mask, nullptr, w.lp64, nullptr, stats, st);
+        launch_logprobs(L, x->dtype, tokens, tokens_are_i64, mask, nullptr, w.lp64, nullptr, stats, w.acc, st);
     }
     pair_kernel<<<(int)(pairs < LAUNCH_ROWS ? pairs : LAUNCH_ROWS), 256, 0, st>>>(w.lp64, mask, ref_logprobs, pairs, x->n_tok, beta, label_smoothing, scale,
                                                 rewards, sd, w.part, pairs == 1 ? loss : nullptr);
@@ -1553,7 +1644,7 @@ extern "C" int ppo_distillation_loss(const ppo_token_logits* x, const void* teac
     if (L.n > 0) {
         count_rows(p.w, x, w, st);
         const size_t lds = teacher_lds(top);
-        const int parts = grad ? split_parts(L, x->dtype) : 0;
+        const int parts = grad ? split_parts(L, x->dtype, 64, 128 * 1024) : 0;
         const Split sp = {w.acc, w.teach, parts};
         BY_TYPE(x->dtype, T, {
             if (!grad && L.n >= 512)
@@ -1562,8 +1653,7 @@ extern "C" int ppo_distillation_loss(const ppo_token_logits* x, const void* teac
                 EACH_LAUNCH(L, false, grid, (distill_forward_kernel<T, MODE_FEW><<<grid, stream_threads(MODE_FEW), lds, st>>>(L, p)))
             else if (parts) {
                 const dim3 grid((unsigned)L.n, parts);
-                split_teacher_kernel<T><<<(unsigned)L.n, 64, lds, st>>>(L, p, sp);
-                split_stats_kernel<T, false><<<grid, 256, 0, st>>>(L, mask, nullptr, 0, sp);
+                split_teacher_kernel<T><<<dim3((unsigned)L.n, parts + 1), 256, lds, st>>>(L, p, sp);
                 distill_split_kernel<T><<<grid, 256, lds, st>>>(L, p, sp);
             } else if (held_in_8(L, x->dtype))
                 EACH_LAUNCH(L, false, grid, (distill_kernel<T, 8><<<grid, held_threads(L, x->dtype, 8), lds, st>>>(L, p)))
@@ -1588,6 +1678,6 @@ extern "C" int ppo_distillation_backward(const ppo_token_logits* x, const void* 
     p.w.mask = mask;
     p.stats = (RowStats*)row_stats;
     p.factor = grad_factor;
-    BY_TYPE(x->dtype, T, EACH_LAUNCH(L, false, grid, (distill_backward_kernel<T><<<grid, 256, teacher_lds(top), (hipStream_t)stream>>>(L, p))))
+    BY_TYPE(x->dtype, T, EACH_LAUNCH(L, false, grid, (distill_backward_kernel<T><<<grid, backward_threads(L, x->dtype), teacher_lds(top), (hipStream_t)stream>>>(L, p))))
     return (int)hipGetLastError();
 }

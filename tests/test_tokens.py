@@ -84,13 +84,13 @@ def test_c_abi_refuses_logits(more, code):
     L, x = _lib.lib(), ctypes.byref(logits_struct(**more))
     at = 1 << 20   # a pointer that is never followed: every call is refused before a launch
     terms = ctypes.byref(_lib.PolicyTerms(0.2, 0.2, 0.0, 0.0, 1.0, 1))
-    assert L.ppo_token_logprobs(x, at, 1, None, at, None, None, None) == code
+    assert L.ppo_token_logprobs(x, at, 1, None, at, None, None, None, 0, None) == code
     assert L.ppo_token_logprobs_backward(x, at, 1, None, at, at, 4, 1, None, 0, 0, None, at, None) == code
     assert L.ppo_policy_loss(x, at, 1, None, at, at, 4, 1, None, terms, at, at, at, None, None, at, at, 1 << 40, None) == code
     assert L.ppo_preference_loss(x, at, 1, None, at, 0.1, 0.0, 1.0, at, at, None, None, at, at, 1 << 40, None) == code
     assert L.ppo_distillation_loss(x, at, 1, at, 0, 4, None, 1, 1.0, at, at, None, at, at, 1 << 40, None) == code
     assert L.ppo_distillation_backward(x, at, 1, at, 0, 4, None, at, None, at, None) == code
-    assert L.ppo_token_logprobs(None, at, 1, None, at, None, None, None) == -1
+    assert L.ppo_token_logprobs(None, at, 1, None, at, None, None, None, 0, None) == -1
 
 
 @pytest.mark.parametrize("more,code", BAD_GRADS)
@@ -118,10 +118,11 @@ def test_c_abi_refuses_other_arguments():
         x, at, 1, at, dtype, top, None, red, 1.0, loss, at, None, None, at, size, None)
     assert distill(0) == -1 and distill(513) == -3 and distill(4, dtype=5) == -1 and distill(4, red=-1) == -1
     assert distill(4, size=need - 1) == -2 and distill(4, loss=None) == -1
-    assert L.ppo_token_logprobs(x, None, 1, None, at, None, None, None) == -1
+    assert L.ppo_token_logprobs(x, None, 1, None, at, None, None, None, 0, None) == -1
+    assert L.ppo_token_logprobs(x, at, 1, None, at, None, None, at, need - 1, None) == -2
     assert L.ppo_token_logprobs_backward(x, at, 1, None, None, at, 4, 1, None, 0, 0, None, at, None) == -1
     empty = ctypes.byref(logits_struct(n_seq=0, data=None))
-    assert L.ppo_token_logprobs(empty, None, 1, None, None, None, None, None) == 0
+    assert L.ppo_token_logprobs(empty, None, 1, None, None, None, None, None, 0, None) == 0
 
 
 def test_constants_are_the_headers():
