@@ -8,9 +8,15 @@
 // Everything a row needs of its V logits is (m, S, E) = (max x, sum e_i, sum e_i u_i) with
 // u_i = (x_i - m) c log2(e), e_i = 2^u_i: lse = c m + ln S, H = ln S - ln2 E / S, p_i = e_i / S.  The three are
 // kept per thread with a running maximum, joined over the workgroup, and the gradient is one multiply-add and a
-// product on each e_i.  u_i is formed as a difference first: it is 0 at the maximum for any size of the logits
-// (c x - c m would leave the rounding of a large c m), and a logit of -inf or of the type's lowest value has
-// e_i = 0.  Sums are fp32 within a thread and over the workgroup, one row's scalars are finished in fp64.
+// product on each e_i.  A logit of -inf or of the type's lowest value has e_i = 0.  Sums are fp32 within a thread and
+// over the workgroup, one row's scalars are finished in fp64.
+//
+// What bounds it: memory.  With entropy and gradient a bf16 logit is 4 bytes of traffic and some 17 instructions (an
+// exponential counts as four), which is half of what the vector units can do while the memory moves it.  So a row is
+// read once and stays on the chip until its gradient is written (policy_kernel, distill_kernel), or, where its gradient
+// waits for other rows or a later call, is read a second time in reverse order, from the cache as far as that reaches.
+// Measured, bf16, whole calls: 4096 rows of 131072 logits with gradient 5.4 TB/s of logits and gradients (a plain copy
+// reaches 5.1 to 5.4), 8184 rows of 50001 forward only 5.9 TB/s (reading alone 6.1 to 6.3).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -324,8 +330,8 @@ __device__ __forceinline__ bool stream_row(const T* x, int V, float c2, float co
 }
 
 // ------------------------------------------------------------------------------------------ a row on the chip
-// A row's threads hold CH vectors each, so that statistics and gradient read memory once: 16 threads of vectors a
-// lane are 64 registers, 1024 threads then hold 256 KB.  Vectors beyond are read again for the gradient.  Vector j
+// A row's threads hold CH vectors each, so that statistics and gradient read memory once: 16 vectors a thread are 64
+// registers, and 1024 threads then hold 256 KB.  Vectors beyond are read again for the gradient.  Vector j
 // belongs to thread (j + shift) % nt; lanes beside the row hold its first or last vector, not counted and not stored.
 template <typename T, int CH> struct Row {
     u32x4 v[CH];
@@ -1117,7 +1123,9 @@ __device__ __forceinline__ RowGrad teacher_seed(const Teacher& s, float m, float
 template <typename T, bool NEAR>
 __device__ __forceinline__ void teacher_places(const TeacherArgs& p, const Teacher& s, T* out, const Logits& L,
                                                const RowGrad& rg, float g, const Span<T>& w, int seg = 0, int segs = 1) {
-    __syncthreads();          // the bulk is written
+    // The bulk is written, and has arrived: other waves' stores to these places come first (no cost was measured).
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
     if (*s.bad) return;
     const int per = piece_of(w, segs);
     for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
@@ -1389,18 +1397,21 @@ static bool by_wave(const Logits& L, int dtype) { return row_bytes(L, dtype) <= 
     }
 
 // Threads of a row that is only read: few, because what is done once a row costs each wave the same, and the chip is
-// full with 256 rows under way and more; all that a workgroup can have where there are fewer rows than that.
+// full with 512 rows under way and more (16384 rows of 16 KB: 48 us with 128 threads, 60 with 256; 4096 rows of 100 KB: 74 and
+// 71); all that a workgroup can have where there are fewer rows than that.
 static int stream_mode(const Logits& L, int dtype) { return by_wave(L, dtype) ? MODE_WAVE : L.n >= 512 ? MODE_BLOCK : MODE_FEW; }
-static int stream_threads(int mode) { return mode == MODE_FEW ? 1024 : 256; }
+static int stream_threads(const Logits& L, int dtype, int mode) {
+    return mode == MODE_FEW ? 1024 : mode == MODE_BLOCK && row_bytes(L, dtype) <= 16384 ? 128 : 256;
+}
 #define BY_MODE(mode, M, ...)                                                      \
     if ((mode) == MODE_WAVE) { constexpr int M = MODE_WAVE; __VA_ARGS__; }         \
     else if ((mode) == MODE_BLOCK) { constexpr int M = MODE_BLOCK; __VA_ARGS__; }  \
     else { constexpr int M = MODE_FEW; __VA_ARGS__; }
 
 // Pieces of a row where there are so few long ones (at most `rows`, of `bytes` at least) that they leave most of the chip
-// idle; 0: the row is not cut.  Device time of bf16 rows of 256 KB, whole / cut: policy loss with gradient 1 row 20 / 7.4 us,
-// 16 rows 22 / 10, 128 rows 29 / 24 (rows of 32 KB: 6.6 / 7); distillation 1 row
-// 20 / 10, 64 rows 26 / 19, 128 rows 29 / 32; log-probabilities 1 row 11 / 5.5, 64 rows 12 / 9, 256 rows 17 / 17.
+// idle; 0: the row is not cut.  Device time of bf16 rows of 256 KB, whole / cut, in us: policy loss with gradient 1 row
+// 20 / 7.4, 16 rows 22 / 10, 128 rows 29 / 24 (100 KB: 12 / 7.6, 15 / 10, 18 / 15; 32 KB: no gain); distillation 1 row 20 / 10,
+// 64 rows 26 / 19, 128 rows 29 / 32; log-probabilities 1 row 11 / 5.5, 64 rows 12 / 9, 256 rows 17 / 17.
 static int split_parts(const Logits& L, int dtype, int64_t rows, int64_t bytes) {
     if (L.n > rows || row_bytes(L, dtype) < bytes) return 0;
     const int64_t most = row_bytes(L, dtype) / 8192, want = 1024 / L.n;
@@ -1459,7 +1470,7 @@ static void launch_logprobs(Logits L, int dtype, const void* tokens, int i64, co
         return;
     }
     BY_TYPE(dtype, T, BY_MODE(stream_mode(L, dtype), MODE, BY_FLAG(entropy != nullptr, ENT, BY_FLAG(stats != nullptr, KEEP, {
-        EACH_LAUNCH(L, MODE == MODE_WAVE, grid, (logprobs_kernel<T, MODE, ENT, KEEP><<<grid, stream_threads(MODE), 0, st>>>(
+        EACH_LAUNCH(L, MODE == MODE_WAVE, grid, (logprobs_kernel<T, MODE, ENT, KEEP><<<grid, stream_threads(L, dtype, MODE), 0, st>>>(
             L, tokens, i64, mask, logprobs, logprobs64, entropy, stats)))
     }))))
 }
@@ -1484,6 +1495,7 @@ extern "C" int ppo_token_logprobs(const ppo_token_logits* x, const void* tokens,
     if (!tokens || !logprobs) return PPO_E_BADARG;
     const Workspace w = carve(workspace, x->n_seq, x->n_tok);
     if (workspace && workspace_bytes < w.bytes) return PPO_E_WORKSPACE;
+    if ((uintptr_t)workspace % 16) return PPO_E_BADARG;
     launch_logprobs(L, x->dtype, tokens, tokens_are_i64, mask, logprobs, nullptr, entropy, (RowStats*)row_stats,
                     workspace ? w.acc : nullptr, (hipStream_t)stream);
     return (int)hipGetLastError();
@@ -1524,6 +1536,7 @@ extern "C" int ppo_policy_loss(const ppo_token_logits* x, const void* tokens, in
     const hipStream_t st = (hipStream_t)stream;
     const Workspace w = carve(workspace, x->n_seq, x->n_tok);
     if (!workspace || workspace_bytes < w.bytes) return PPO_E_WORKSPACE;
+    if ((uintptr_t)workspace % 16) return PPO_E_BADARG;
     Logits L = logits_of(x, grad);
     PolicyArgs p;
     bool solo = false;
@@ -1554,7 +1567,7 @@ extern "C" int ppo_policy_loss(const ppo_token_logits* x, const void* tokens, in
         count_rows(p.w, x, w, st);
         if (!grad) {
             BY_TYPE(x->dtype, T, BY_MODE(stream_mode(L, x->dtype), MODE, {
-                const int threads = solo && MODE == MODE_WAVE ? 64 * (int)L.n : stream_threads(MODE);
+                const int threads = solo && MODE == MODE_WAVE ? 64 * (int)L.n : stream_threads(L, x->dtype, MODE);
                 EACH_LAUNCH(L, MODE == MODE_WAVE, grid, (policy_forward_kernel<T, MODE><<<solo ? 1 : grid, threads, 0, st>>>(L, p)))
             }))
         } else if (const int parts = split_parts(L, x->dtype, 128, 64 * 1024)) {
@@ -1589,6 +1602,7 @@ extern "C" int ppo_preference_loss(const ppo_token_logits* x, const void* tokens
     const hipStream_t st = (hipStream_t)stream;
     const Workspace w = carve(workspace, x->n_seq, x->n_tok);
     if (!workspace || workspace_bytes < w.bytes) return PPO_E_WORKSPACE;
+    if ((uintptr_t)workspace % 16) return PPO_E_BADARG;
     Logits L = logits_of(x, grad);
     if (L.n > 0 && !tokens) return PPO_E_BADARG;
     const int64_t pairs = x->n_seq / 2;
@@ -1634,6 +1648,7 @@ extern "C" int ppo_distillation_loss(const ppo_token_logits* x, const void* teac
     const hipStream_t st = (hipStream_t)stream;
     const Workspace w = carve(workspace, x->n_seq, x->n_tok);
     if (!workspace || workspace_bytes < w.bytes) return PPO_E_WORKSPACE;
+    if ((uintptr_t)workspace % 16) return PPO_E_BADARG;
     e = weights_of(&p.w, mask, reduction, scale, x, w);
     if (e) return e;
     Logits L = logits_of(x, grad);
@@ -1648,9 +1663,9 @@ extern "C" int ppo_distillation_loss(const ppo_token_logits* x, const void* teac
         const Split sp = {w.acc, w.teach, parts};
         BY_TYPE(x->dtype, T, {
             if (!grad && L.n >= 512)
-                EACH_LAUNCH(L, false, grid, (distill_forward_kernel<T, MODE_BLOCK><<<grid, stream_threads(MODE_BLOCK), lds, st>>>(L, p)))
+                EACH_LAUNCH(L, false, grid, (distill_forward_kernel<T, MODE_BLOCK><<<grid, stream_threads(L, x->dtype, MODE_BLOCK), lds, st>>>(L, p)))
             else if (!grad)
-                EACH_LAUNCH(L, false, grid, (distill_forward_kernel<T, MODE_FEW><<<grid, stream_threads(MODE_FEW), lds, st>>>(L, p)))
+                EACH_LAUNCH(L, false, grid, (distill_forward_kernel<T, MODE_FEW><<<grid, stream_threads(L, x->dtype, MODE_FEW), lds, st>>>(L, p)))
             else if (parts) {
                 const dim3 grid((unsigned)L.n, parts);
                 split_teacher_kernel<T><<<dim3((unsigned)L.n, parts + 1), 256, lds, st>>>(L, p, sp);

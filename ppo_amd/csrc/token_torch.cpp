@@ -376,9 +376,9 @@ static Policy3 policy_loss(const Tensor& x, const Tensor& tokens, const Tensor& 
 
 // The version counter of overwritten memory moves, so that autograd notices a use of old values.
 static void overwritten(const OptTensor& out, const Tensor& x) {
-    if (!out) return;
-    torch::autograd::impl::bump_version(*out);
-    if (out->data_ptr() == x.data_ptr()) torch::autograd::impl::bump_version(x);
+    if (!out) return;         // (tensors of inference mode have no counter)
+    if (!out->is_inference()) torch::autograd::impl::bump_version(*out);
+    if (out->data_ptr() == x.data_ptr() && !x.is_inference()) torch::autograd::impl::bump_version(x);
 }
 
 static std::tuple<Tensor, Tensor, Tensor, Tensor> policy_loss_and_grad(

@@ -547,6 +547,73 @@ def test_overwritten_logits_are_noticed_by_autograd():
         square.sum().backward()
 
 
+def calls(x, y, m):
+    """The differentiable losses as functions of the logits."""
+    z = torch.full(y.shape, -2.0, device="cuda")
+    return [lambda a: K().token_logprobs(a, y, m)[0].sum(), lambda a: K().token_logprobs(a, y, m)[1].sum(),
+            lambda a: K().policy_loss(a, y, z, z, m, ref_logprobs=z, kl_coef=0.1, entropy_coef=0.1)[0],
+            lambda a: K().preference_loss(a, y, z.sum(-1), m)[0],
+            lambda a: K().distillation_loss(a, y[..., None], z[..., None], m)[0]]
+
+
+def test_autograd_corners():
+    """Backward twice over a kept graph, a gradient of a gradient (refused, and only when it is asked for), logits changed
+    in between (noticed), and saved tensors that leave the GPU in between."""
+    x, y, m = make(15, 2, 5, 700, torch.float32)
+    for fn in calls(x, y, m):
+        a = x.clone().requires_grad_(True)
+        loss = fn(a)
+        one = torch.autograd.grad(loss, a, retain_graph=True)[0]
+        two = torch.autograd.grad(loss * 2, a, create_graph=True)[0]
+        assert torch.equal(one * 2, two.detach())
+        with pytest.raises(RuntimeError, match="differentiated once"):
+            two.sum().backward()
+        b = x.clone().requires_grad_(True)
+        c = b * 1.0
+        loss = fn(c)
+        c.mul_(2.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        with torch.autograd.graph.save_on_cpu():
+            loss = fn(a)
+        held = [torch.full((1 << 20,), float("nan"), device="cuda") for _ in range(8)]   # what was freed is written over
+        assert torch.equal(torch.autograd.grad(loss, a)[0], one)
+        del held
+        with torch.inference_mode():
+            assert torch.equal(fn(x), fn(x.clone()))
+    with torch.inference_mode():
+        a, z = x.clone(), torch.full(y.shape, -2.0, device="cuda")
+        want = K().policy_loss_and_grad(x, y, z, z, m)[1]
+        assert torch.equal(K().policy_loss_and_grad(a, y, z, z, m, out=a)[1], want) and torch.equal(a, want)
+
+
+def test_gradients_on_a_side_stream():
+    """A forward and a backward pass on a stream of its own, between work on the default stream."""
+    x, y, m = make(16, 4, 30, 4099, torch.bfloat16)
+    want = [torch.autograd.grad(fn(a), a)[0] for fn, a in ((f, x.clone().requires_grad_(True)) for f in calls(x, y, m))]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [torch.autograd.grad(fn(a), a)[0] for fn, a in ((f, x.clone().requires_grad_(True)) for f in calls(x, y, m))]
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.bfloat16, torch.float16])
+def test_other_types_beside_the_logits(dtype):
+    x, y, m = make(17, 2, 4, 300, torch.float16)
+    z = torch.linspace(-4, -1, 8, device="cuda").view(2, 4).to(dtype)
+    a = K().policy_loss_and_grad(x, y, z, z, m, ref_logprobs=z, kl_coef=0.1)
+    f = z.float()
+    b = K().policy_loss_and_grad(x, y.int(), f, f.t().contiguous().t(), m.to(torch.uint8) * 7, ref_logprobs=f, kl_coef=0.1)
+    for p, q in zip(a, b):
+        assert torch.equal(p, q)
+    a, b = K().preference_loss_and_grad(x, y, z[:, 0], m), K().preference_loss_and_grad(x, y, f[:, 0], m)
+    for p, q in zip(a, b):
+        assert torch.equal(p, q)
+
+
 def test_far_rows():
     """Offsets beyond 2^31 elements, in the logits and in the gradient."""
     v, far = 1003, (1 << 31) + 24
