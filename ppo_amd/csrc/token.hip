@@ -919,6 +919,132 @@ __global__ __launch_bounds__(1024, 4) void policy_kernel(Logits L, PolicyArgs p)
     row_loss<WAVE>(p, r, L.n, weighted_loss(p, d.o, d.h));
 }
 
+// Rows of at most 256 logits, as of a head of a few actions: G lanes a row (4 up to 64 logits, 16 beyond), 16 logits a lane
+// at most, element by element.  A wave's fp64 arithmetic then serves 64 / G rows: 524288 rows of 6 logits with their
+// gradient took 413 us with a wave each.
+template <typename T, int G> struct Tiny {
+    float f[16];
+    int lane;
+
+    __device__ __forceinline__ Acc load(const T* x, int V, float c2) {
+        lane = threadIdx.x & (G - 1);
+        Acc a = acc_empty();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            f[k] = -__builtin_inff();
+            if (k * G + lane < V) f[k] = wide(x[k * G + lane]);
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) a.m = fmaxf(a.m, f[k]);
+        a.m = group(a.m, [](float p, float q) { return fmaxf(p, q); });
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+            if (k * G < V) acc_add<true>(a, f[k], c2);
+        a.s = group(a.s, [](float p, float q) { return p + q; });
+        a.e = group(a.e, [](float p, float q) { return p + q; });
+        return a;
+    }
+    // over the G lanes of a row, the same bits in each
+    template <typename F> static __device__ __forceinline__ float group(float v, F op) {
+        if (G == 16) {
+            v = op(v, ror<0x128>(v));
+            v = op(v, ror<0x124>(v));
+        }
+        v = op(v, ror<0x4e>(v));   // quads: lanes 2, 3, 0, 1
+        return op(v, ror<0xb1>(v));   // lanes 1, 0, 3, 2
+    }
+    __device__ __forceinline__ void store(T* out, int V, float c2, const RowGrad& g) const {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int i = k * G + lane;
+            if (i < V) {
+                const float d = grad_of<true, false>(g, f[k], c2);
+                out[i] = (T)(i == g.tok ? d + g.gt : d);
+            }
+        }
+    }
+    static __device__ __forceinline__ void zero(T* out, int V) {
+        for (int i = threadIdx.x & (G - 1); i < V; i += G) out[i] = (T)0.0f;
+    }
+    static __device__ __forceinline__ int64_t row(const Logits& L) {
+        return L.r0 + ((int64_t)blockIdx.x * 256 + threadIdx.x) / G;
+    }
+};
+
+template <typename T, int G>
+__global__ __launch_bounds__(256) void tiny_logprobs_kernel(Logits L, const void* tokens, int i64, const uint8_t* mask,
+                                                            float* logprobs, double* logprobs64, float* entropy, RowStats* stats) {
+    const int64_t r = Tiny<T, G>::row(L);
+    if (r >= L.n) return;
+    double lp = 0.0;
+    RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
+    if (!mask || mask[r]) {
+        const T* x = row_in<T>(L, place_of(L, r));
+        Tiny<T, G> row;
+        const Acc a = row.load(x, L.V, L.c2);
+        const double ln_s = ln_sum<true>(L, a);
+        lp = logp_of<false>(L, token_logit(x, int_at(tokens, i64, r), L.V), a.m, ln_s);
+        st = {a.m, a.s, entropy_of(L, a, ln_s), 0.0f};
+    }
+    if (threadIdx.x & (G - 1)) return;
+    if (logprobs) logprobs[r] = (float)lp;
+    if (logprobs64) logprobs64[r] = lp;
+    if (entropy) entropy[r] = st.h;
+    if (stats) stats[r] = st;
+}
+
+template <typename T, int G>
+__global__ __launch_bounds__(256) void tiny_backward_kernel(Logits L, const void* tokens, int i64, const uint8_t* mask,
+                                                            const RowStats* __restrict__ stats, Incoming in) {
+    const int64_t r = Tiny<T, G>::row(L);
+    if (r >= L.n) return;
+    const Place at = place_of(L, r);
+    if (mask && !mask[r]) {
+        Tiny<T, G>::zero(row_out<T>(L, at), L.V);
+        return;
+    }
+    Tiny<T, G> row;
+    row.load(row_in<T>(L, at), L.V, L.c2);
+    const float f = in.factor ? *in.factor : 1.0f;
+    const RowStats st = stats[r];
+    const float g_lp = in.lp ? f * in.lp[at.b * in.lp_s + at.t * in.lp_t] : 0.0f;
+    const float g_h = in.h ? f * in.h[at.b * in.h_s + at.t * in.h_t] : 0.0f;
+    row.store(row_out<T>(L, at), L.V, L.c2,
+              grad_seed(L, st.m, st.s, st.h, in.h ? (float)ln_of(st.s) : 0.0f, g_lp, g_h, int_at(tokens, i64, r)));
+}
+
+// Loss, and the gradient (GRAD) or what a backward pass needs.
+template <typename T, int G, bool GRAD>
+__global__ __launch_bounds__(256) void tiny_policy_kernel(Logits L, PolicyArgs p) {
+    const int64_t r = Tiny<T, G>::row(L);
+    if (r >= L.n) return;
+    const Place at = place_of(L, r);
+    PolicyDone d = {};
+    RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
+    if (!p.w.mask || p.w.mask[r]) {
+        const T* x = row_in<T>(L, at);
+        const PolicyIn in = policy_in(L, p, x, r, at);
+        Tiny<T, G> row;
+        const Acc a = row.load(x, L.V, L.c2);
+        d = policy_done<false>(L, p, in, a, at, 0.0f);
+        st = {a.m, a.s, d.h, 0.0f};
+        if (GRAD) row.store(row_out<T>(L, at), L.V, L.c2, policy_seed(L, d, a.m, a.s, in.tok));
+    } else if (GRAD) {
+        Tiny<T, G>::zero(row_out<T>(L, at), L.V);
+    }
+    if (threadIdx.x & (G - 1)) return;
+    p.logprobs[r] = (float)d.lp;
+    if (p.entropy) p.entropy[r] = d.h;
+    if (!GRAD && p.stats) {
+        p.stats[r] = st;
+        p.g_lp[r] = d.o.g_lp;
+        p.g_h[r] = d.o.g_h;
+    }
+    const double loss = weighted_loss(p, d.o, d.h);
+    if (p.solo) *p.solo = (float)loss;     // the only row
+    else p.part[r] = loss;
+}
+
 // Few long rows: a row in `parts` pieces of a workgroup each, first their statistics (split_stats_kernel), then, in a
 // second launch, the row's loss and the pieces' gradients.  The first launch also takes along what of the logits the
 // second needs beside its piece, which another workgroup of that launch may have overwritten.
@@ -1381,6 +1507,12 @@ static Logits logits_of(const ppo_token_logits* x, void* grad) {
 
 static int64_t row_bytes(const Logits& L, int dtype) { return (int64_t)L.V * (dtype == PPO_F32 ? 4 : 2); }
 
+// Lanes of a row of so few logits that several share a wave; 0: more than that.
+static int tiny_lanes(const Logits& L) { return L.V <= 64 ? 4 : L.V <= 256 ? 16 : 0; }
+#define BY_LANES(lanes, G, ...)                                                    \
+    if ((lanes) == 4) { constexpr int G = 4; __VA_ARGS__; }                        \
+    else { constexpr int G = 16; __VA_ARGS__; }
+
 // A wave takes a row of up to 4 KB by itself: its 64 lanes hold that in four vectors each.
 static bool by_wave(const Logits& L, int dtype) { return row_bytes(L, dtype) <= 4096; }
 
@@ -1395,6 +1527,8 @@ static bool by_wave(const Logits& L, int dtype) { return row_bytes(L, dtype) <= 
         const int grid = WAVE ? (rows_ + 3) / 4 : rows_;                           \
         __VA_ARGS__;                                                               \
     }
+
+#define EACH_TINY(L, G, grid, ...) EACH_LAUNCH(L, false, rows, { const int grid = (rows + 256 / G - 1) / (256 / G); __VA_ARGS__; })
 
 // Threads of a row that is only read: few, because what is done once a row costs each wave the same, and the chip is
 // full with 512 rows under way and more (16384 rows of 16 KB: 48 us with 128 threads, 60 with 256; 4096 rows of 100 KB: 74 and
@@ -1469,6 +1603,11 @@ static void launch_logprobs(Logits L, int dtype, const void* tokens, int i64, co
         })
         return;
     }
+    if (const int lanes = tiny_lanes(L)) {
+        BY_TYPE(dtype, T, BY_LANES(lanes, G, EACH_TINY(L, G, grid, (tiny_logprobs_kernel<T, G><<<grid, 256, 0, st>>>(
+            L, tokens, i64, mask, logprobs, logprobs64, entropy, stats)))))
+        return;
+    }
     BY_TYPE(dtype, T, BY_MODE(stream_mode(L, dtype), MODE, BY_FLAG(entropy != nullptr, ENT, BY_FLAG(stats != nullptr, KEEP, {
         EACH_LAUNCH(L, MODE == MODE_WAVE, grid, (logprobs_kernel<T, MODE, ENT, KEEP><<<grid, stream_threads(L, dtype, MODE), 0, st>>>(
             L, tokens, i64, mask, logprobs, logprobs64, entropy, stats)))
@@ -1503,6 +1642,11 @@ extern "C" int ppo_token_logprobs(const ppo_token_logits* x, const void* tokens,
 
 static int launch_backward(Logits L, int dtype, const void* tokens, int i64, const uint8_t* mask,
                            const RowStats* stats, const Incoming& in, hipStream_t st) {
+    if (const int lanes = tiny_lanes(L)) {
+        BY_TYPE(dtype, T, BY_LANES(lanes, G, EACH_TINY(L, G, grid, (tiny_backward_kernel<T, G><<<grid, 256, 0, st>>>(
+            L, tokens, i64, mask, stats, in)))))
+        return (int)hipGetLastError();
+    }
     BY_TYPE(dtype, T, BY_FLAG(by_wave(L, dtype), WAVE, BY_FLAG(in.h != nullptr, ENT, {
         EACH_LAUNCH(L, WAVE, grid, (backward_kernel<T, WAVE, ENT><<<dim3(grid, WAVE ? 1 : backward_parts(L, dtype)), WAVE ? 256 : backward_threads(L, dtype), 0, st>>>(
             L, tokens, i64, mask, stats, in)))
@@ -1562,10 +1706,16 @@ extern "C" int ppo_policy_loss(const ppo_token_logits* x, const void* tokens, in
         p.g_h = seeds ? seeds + L.n : nullptr;
         p.part = w.part;
         // One workgroup, of a wave for each row, where that takes them all: the loss then needs no second launch.
-        solo = L.n == 1 || (by_wave(L, x->dtype) && L.n <= SOLO_ROWS);
+        const int lanes = tiny_lanes(L);
+        solo = L.n == 1 || (!lanes && by_wave(L, x->dtype) && L.n <= SOLO_ROWS);
         p.solo = solo ? loss : nullptr;
+        if (lanes) p.w.count_here = 0;
         count_rows(p.w, x, w, st);
-        if (!grad) {
+        if (lanes) {
+            BY_TYPE(x->dtype, T, BY_LANES(lanes, G, BY_FLAG(grad != nullptr, GRAD, {
+                EACH_TINY(L, G, grid, (tiny_policy_kernel<T, G, GRAD><<<grid, 256, 0, st>>>(L, p)))
+            })))
+        } else if (!grad) {
             BY_TYPE(x->dtype, T, BY_MODE(stream_mode(L, x->dtype), MODE, {
                 const int threads = solo && MODE == MODE_WAVE ? 64 * (int)L.n : stream_threads(L, x->dtype, MODE);
                 EACH_LAUNCH(L, MODE == MODE_WAVE, grid, (policy_forward_kernel<T, MODE><<<solo ? 1 : grid, threads, 0, st>>>(L, p)))
