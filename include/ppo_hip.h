@@ -349,7 +349,7 @@ typedef struct {
     int64_t grad_seq_stride, grad_tok_stride; /* of the gradient, where one is written */
     int64_t n_seq, n_tok, vocab;
     int dtype;                                /* PPO_F32, PPO_BF16 or PPO_F16 */
-    float inv_temperature;                    /* probabilities are softmax(logits * inv_temperature) */
+    double inv_temperature;                   /* probabilities are softmax(logits * inv_temperature) */
 } ppo_token_logits;
 
 size_t ppo_token_workspace_bytes(int64_t n_seq, int64_t n_tok);

@@ -18,7 +18,7 @@ class TokenLogits(ctypes.Structure):
     """ppo_token_logits"""
     _fields_ = [("data", c_void_p), ("seq_stride", c_int64), ("tok_stride", c_int64), ("grad_seq_stride", c_int64),
                 ("grad_tok_stride", c_int64), ("n_seq", c_int64), ("n_tok", c_int64), ("vocab", c_int64),
-                ("dtype", c_int), ("inv_temperature", c_float)]
+                ("dtype", c_int), ("inv_temperature", c_double)]
 
 
 class PolicyTerms(ctypes.Structure):

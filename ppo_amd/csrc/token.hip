@@ -22,7 +22,6 @@
 
 #include "../../include/ppo_hip.h"
 
-#define LOG2E_F 1.4426950408889634f
 #define LN2_D 0.6931471805599453
 #define U_FLOOR (-1.0e6f)    // below it e_i is 0: products e_i u_i take this in place of -inf
 
@@ -120,14 +119,18 @@ template <bool ENT, bool NEAR = false> __device__ __forceinline__ void acc_rebas
     a.m = mn;
 }
 
-template <bool ENT, bool NEAR = false> __device__ __forceinline__ void acc_add(Acc& a, float x, float c2) {   // a.m >= x, or x is NaN
-    const float u = NEAR ? fmaf(x, c2, -near_max(a.m, c2)) : (x - a.m) * c2;
-    const float e = __builtin_amdgcn_exp2f(u);
+template <bool NEAR> __device__ __forceinline__ float u_of(float x, float m, float c2) {   // m >= x, or x is NaN
+    return NEAR ? fmaf(x, c2, -near_max(m, c2)) : (x - m) * c2;
+}
+template <bool ENT, bool NEAR = false> __device__ __forceinline__ void acc_add(Acc& a, float x, float c2) {
+    const float u = u_of<NEAR>(x, a.m, c2), e = __builtin_amdgcn_exp2f(u);
     a.s += e;
     if (ENT) a.e = fmaf(e, fmaxf(u, U_FLOOR), a.e);
 }
 
-// 16 * M bytes of logits at once: their maximum, one rescaling, their terms
+// 16 * M bytes of logits at once: their maximum, one rescaling, their terms.  The terms are summed by themselves and then
+// added: one by one the many small terms of a long row are below half a step of a sum that has grown, and S comes out
+// too small (131072 normal logits of deviation 5: ln p too large by 6e-7 in the mean).
 template <typename T, int M, bool ENT, bool NEAR = false>
 __device__ __forceinline__ void acc_vecs(Acc& a, const u32x4* v, float c2) {
     constexpr int N = VEC<T>;
@@ -137,8 +140,15 @@ __device__ __forceinline__ void acc_vecs(Acc& a, const u32x4* v, float c2) {
 #pragma unroll
     for (int i = 0; i < N * M; ++i) mx = fmaxf(mx, f[i]);
     acc_rebase<ENT, NEAR>(a, mx, c2);
+    float s, e;
 #pragma unroll
-    for (int i = 0; i < N * M; ++i) acc_add<ENT, NEAR>(a, f[i], c2);
+    for (int i = 0; i < N * M; ++i) {
+        const float u = u_of<NEAR>(f[i], mx, c2), t = __builtin_amdgcn_exp2f(u);
+        s = i ? s + t : t;
+        if (ENT) e = i ? fmaf(t, fmaxf(u, U_FLOOR), e) : t * fmaxf(u, U_FLOOR);
+    }
+    a.s += s;
+    if (ENT) a.e += e;
 }
 
 // The sums as they are relative to m c2 itself: with rho = m c2 - M the terms are e_i 2^-rho, u_i - rho.
@@ -480,7 +490,7 @@ struct Logits {
     int64_t r0;               // first row of this launch
     int V;
     float c, c2;              // 1/temperature; the same times log2(e)
-    double ln2;               // c / c2
+    double ln2;               // 1/temperature / c2
     bool past;                // the gradient is stored past the caches
 };
 
@@ -566,7 +576,7 @@ template <typename T> __device__ __forceinline__ float token_logit(const T* x, i
     return tok >= 0 && tok < V ? wide(x[tok]) : __builtin_nanf("");
 }
 // ln S and ln p of a logit.  c2 is rounded: relative to 1/temperature all u_i are too long by the same factor, which
-// L.ln2 = c / c2 takes back from a single u, and, to first order, E / S from ln S.
+// L.ln2 takes back from a single u, and, to first order, E / S from ln S.
 template <bool ENT> __device__ __forceinline__ double ln_sum(const Logits& L, const Acc& a) {
     const double ln_s = ln_of(a.s);
     return ENT ? fma(L.ln2 - LN2_D, (double)(a.e / a.s), ln_s) : ln_s;
@@ -1462,7 +1472,7 @@ extern "C" size_t ppo_token_workspace_bytes(int64_t n_seq, int64_t n_tok) {
 static int check_logits(const ppo_token_logits* x, const void* grad) {
     if (!x || x->n_seq < 0 || x->n_tok < 0 || x->vocab < 1) return PPO_E_BADARG;
     if (x->dtype != PPO_F32 && x->dtype != PPO_BF16 && x->dtype != PPO_F16) return PPO_E_BADARG;
-    if (!(x->inv_temperature > 0.0f) || !(x->inv_temperature < 1e30f)) return PPO_E_BADARG;
+    if (!(x->inv_temperature > 1e-30) || !(x->inv_temperature < 1e30)) return PPO_E_BADARG;
     if (x->vocab > PPO_MAX_VOCAB || (x->n_tok > 0 && x->n_seq > PPO_MAX_TOKENS / x->n_tok) || x->n_seq > PPO_MAX_TOKENS)
         return PPO_E_UNSUPPORTED;
     const int64_t n = x->n_seq * x->n_tok;
@@ -1488,9 +1498,9 @@ static Logits logits_of(const ppo_token_logits* x, void* grad) {
     L.n = x->n_seq * x->n_tok;
     L.r0 = 0;
     L.V = (int)x->vocab;
-    L.c = x->inv_temperature;
-    L.c2 = x->inv_temperature * LOG2E_F;
-    L.ln2 = (double)L.c / (double)L.c2;
+    L.c = (float)x->inv_temperature;
+    L.c2 = (float)(x->inv_temperature / LN2_D);
+    L.ln2 = x->inv_temperature / (double)L.c2;
     // A gradient that the 256 MB cache cannot hold is stored past it: 32768 bf16 logits a row, loss and gradient and a
     // copy of the gradient after it take 200 us against 208 at 256 MB, but 99 against 81 at 128 MB.
     L.past = L.n * L.V * (x->dtype == PPO_F32 ? 4 : 2) > (int64_t)192 << 20;

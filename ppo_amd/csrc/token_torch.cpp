@@ -108,9 +108,9 @@ static Tensor floats(const Tensor& x, const Tensor& t, const char* name, at::Int
     return t.scalar_type() == at::kFloat ? t : t.to(at::kFloat);
 }
 
-static float inverse(double temperature) {
+static double inverse(double temperature) {
     TORCH_CHECK_VALUE(temperature >= 1e-6 && temperature <= 1e6, "temperature ", temperature, ": between 1e-6 and 1e6 is expected");
-    return (float)(1.0 / temperature);
+    return 1.0 / temperature;
 }
 
 struct Strides {
@@ -167,7 +167,7 @@ static Tensor grad_like(const Tensor& x) {
     return at::empty({reach + lead}, x.options()).as_strided(x.sizes(), x.strides(), lead);
 }
 
-static ppo_token_logits rows_of(const Tensor& x, float inv_t, const Tensor& grad = Tensor()) {
+static ppo_token_logits rows_of(const Tensor& x, double inv_t, const Tensor& grad = Tensor()) {
     ppo_token_logits r{};
     const bool three = x.dim() == 3;
     r.data = x.data_ptr();
@@ -223,7 +223,7 @@ static Tensor once(const Tensor& grad) {
     return (*error)({grad.detach().requires_grad_(true)})[0];
 }
 
-static Tensor backward_call(const Tensor& x, const Tensor& tokens, const Tensor& mask, float inv_t, const float* stats,
+static Tensor backward_call(const Tensor& x, const Tensor& tokens, const Tensor& mask, double inv_t, const float* stats,
                             const float* g_lp, Strides lp, const float* g_ent, Strides ent, const Tensor& factor) {
     const Call call(x);
     const Tensor grad = grad_like(x);
@@ -236,7 +236,7 @@ static Tensor backward_call(const Tensor& x, const Tensor& tokens, const Tensor&
 // ------------------------------------------------------------------------------------------ log-probabilities
 struct Logprobs : torch::CustomClassHolder {
     Tensor tokens, mask;
-    float inv_t = 1.0f;
+    double inv_t = 1.0;
     bool entropy = true;
 };
 
@@ -255,7 +255,7 @@ struct LogprobsNode : torch::autograd::Function<LogprobsNode> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const c10::intrusive_ptr<Logprobs>& p) {
         const Tensor stats = new_floats(x, {p->tokens.numel(), 4});
         const auto [lp, ent] = logprobs_call(x, *p, stats);
-        ctx->saved_data["inv_t"] = (double)p->inv_t;
+        ctx->saved_data["inv_t"] = p->inv_t;
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({x, p->tokens, p->mask, stats});
         if (p->entropy) return {lp, ent};
@@ -266,7 +266,7 @@ struct LogprobsNode : torch::autograd::Function<LogprobsNode> {
         if (!g_lp.defined() && !g_ent.defined()) return variable_list(2);
         const auto s = ctx->get_saved_variables();
         const Strides none{0, 0};
-        return {backward_call(s[0], s[1], s[2], (float)ctx->saved_data["inv_t"].toDouble(), at_of<float>(s[3]),
+        return {backward_call(s[0], s[1], s[2], ctx->saved_data["inv_t"].toDouble(), at_of<float>(s[3]),
                               at_of<float>(g_lp), g_lp.defined() ? row_strides(g_lp) : none, at_of<float>(g_ent),
                               g_ent.defined() ? row_strides(g_ent) : none, Tensor()),
                 Tensor()};
@@ -294,7 +294,7 @@ struct Policy : torch::CustomClassHolder {
     Tensor tokens, mask, old_lp, adv, ref;
     Strides adv_strides{};
     ppo_policy_terms terms{};
-    float inv_t = 1.0f;
+    double inv_t = 1.0;
 };
 
 static c10::intrusive_ptr<Policy> policy_args(const Tensor& x, const Tensor& tokens, const Tensor& old_lp, const Tensor& adv,
@@ -343,7 +343,7 @@ struct PolicyNode : torch::autograd::Function<PolicyNode> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const c10::intrusive_ptr<Policy>& p) {
         const PolicyOut o = policy_call(x, *p, Tensor(), true);
         ctx->saved_data["offset"] = o.ws.need;
-        ctx->saved_data["inv_t"] = (double)p->inv_t;
+        ctx->saved_data["inv_t"] = p->inv_t;
         ctx->saved_data["entropy"] = p->terms.entropy_coef != 0.0f;
         ctx->mark_non_differentiable({o.lp, o.ent});
         ctx->save_for_backward({x, p->tokens, p->mask, o.ws.memory});
@@ -355,7 +355,7 @@ struct PolicyNode : torch::autograd::Function<PolicyNode> {
         const float* stats = (const float*)((const char*)s[3].data_ptr() + ctx->saved_data["offset"].toInt());
         const float* g_lp = stats + 4 * tokens.numel();
         const Strides dense = row_strides(tokens);
-        return {backward_call(x, tokens, s[2], (float)ctx->saved_data["inv_t"].toDouble(), stats, g_lp, dense,
+        return {backward_call(x, tokens, s[2], ctx->saved_data["inv_t"].toDouble(), stats, g_lp, dense,
                               ctx->saved_data["entropy"].toBool() ? g_lp + tokens.numel() : nullptr, dense, g[0]),
                 Tensor()};
     }
@@ -519,7 +519,7 @@ struct TeacherNode : torch::autograd::Function<TeacherNode> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const c10::intrusive_ptr<Teacher>& p) {
         const TeacherOut o = teacher_call(x, *p, Tensor(), true);
         ctx->saved_data["offset"] = o.ws.need;
-        ctx->saved_data["inv_t"] = (double)p->inv_t;
+        ctx->saved_data["inv_t"] = p->inv_t;
         ctx->mark_non_differentiable({o.each});
         ctx->save_for_backward({x, p->index, p->logits, p->mask, o.ws.memory});
         return {o.loss, o.each};
@@ -530,7 +530,7 @@ struct TeacherNode : torch::autograd::Function<TeacherNode> {
         const float* stats = (const float*)((const char*)s[4].data_ptr() + ctx->saved_data["offset"].toInt());
         const Call call(x);
         const Tensor grad = grad_like(x);
-        const ppo_token_logits r = rows_of(x, (float)ctx->saved_data["inv_t"].toDouble(), grad);
+        const ppo_token_logits r = rows_of(x, ctx->saved_data["inv_t"].toDouble(), grad);
         done(lib.ppo_distillation_backward(&r, index.data_ptr(), is_i64(index), values.data_ptr(), type_code(values.scalar_type()),
                                            (int)index.size(-1), at_of<uint8_t>(s[3]), stats, at_of<float>(g[0]), grad.data_ptr(),
                                            call.stream));
