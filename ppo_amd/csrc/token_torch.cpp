@@ -346,10 +346,12 @@ struct PolicyNode : torch::autograd::Function<PolicyNode> {
         ctx->saved_data["inv_t"] = p->inv_t;
         ctx->saved_data["entropy"] = p->terms.entropy_coef != 0.0f;
         ctx->mark_non_differentiable({o.lp, o.ent});
+        ctx->set_materialize_grads(false);    // else two launches fill zeros that nobody reads
         ctx->save_for_backward({x, p->tokens, p->mask, o.ws.memory});
         return {o.loss, o.lp, o.ent};
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
+        if (!g[0].defined()) return variable_list(2);
         const auto s = ctx->get_saved_variables();
         const Tensor &x = s[0], &tokens = s[1];
         const float* stats = (const float*)((const char*)s[3].data_ptr() + ctx->saved_data["offset"].toInt());
@@ -441,10 +443,12 @@ struct PreferenceNode : torch::autograd::Function<PreferenceNode> {
         const PreferenceOut o = preference_call(x, *p, Tensor(), true);
         ctx->saved_data["offset"] = o.ws.need;
         ctx->mark_non_differentiable({o.rewards});
+        ctx->set_materialize_grads(false);
         ctx->save_for_backward({x, p->tokens, p->mask, o.ws.memory, o.seeds});
         return {o.loss, o.rewards};
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
+        if (!g[0].defined()) return variable_list(2);
         const auto s = ctx->get_saved_variables();
         const float* stats = (const float*)((const char*)s[3].data_ptr() + ctx->saved_data["offset"].toInt());
         return {backward_call(s[0], s[1], s[2], 1.0f, stats, at_of<float>(s[4]), {1, 0}, nullptr, {0, 0}, g[0]), Tensor()};
@@ -521,10 +525,12 @@ struct TeacherNode : torch::autograd::Function<TeacherNode> {
         ctx->saved_data["offset"] = o.ws.need;
         ctx->saved_data["inv_t"] = p->inv_t;
         ctx->mark_non_differentiable({o.each});
+        ctx->set_materialize_grads(false);
         ctx->save_for_backward({x, p->index, p->logits, p->mask, o.ws.memory});
         return {o.loss, o.each};
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
+        if (!g[0].defined()) return variable_list(2);
         const auto s = ctx->get_saved_variables();
         const Tensor &x = s[0], &index = s[1], &values = s[2];
         const float* stats = (const float*)((const char*)s[4].data_ptr() + ctx->saved_data["offset"].toInt());
