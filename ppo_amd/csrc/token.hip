@@ -11,12 +11,12 @@
 // product on each e_i.  A logit of -inf or of the type's lowest value has e_i = 0.  Sums are fp32 within a thread and
 // over the workgroup, one row's scalars are finished in fp64.
 //
-// What bounds it: memory.  With entropy and gradient a bf16 logit is 4 bytes of traffic and some 17 instructions (an
-// exponential counts as four), which is half of what the vector units can do while the memory moves it.  So a row is
+// What bounds it: memory.  With gradient a bf16 logit is 4 bytes of traffic and the time of some 16 instructions (10, of
+// which two exponentials count as four each), two thirds of what the vector units can do while the memory moves it.  So a row is
 // read once and stays on the chip until its gradient is written (policy_kernel, distill_kernel), or, where its gradient
 // waits for other rows or a later call, is read a second time in reverse order, from the cache as far as that reaches.
 // Measured, bf16, whole calls: 4096 rows of 131072 logits with gradient 5.4 TB/s of logits and gradients (a plain copy
-// reaches 5.1 to 5.4), 8184 rows of 50001 forward only 5.9 TB/s (reading alone 6.1 to 6.3).
+// reaches 5.1 to 5.4), 8184 rows of 50001 forward only 6.2 TB/s (reading alone 6.1 to 6.3).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -309,7 +309,7 @@ __device__ __forceinline__ Acc stream_stats(const T* body, int nvec, float edge,
 }
 
 // How a forward-only kernel reads its rows: a wave each; a workgroup each; a workgroup each where there are so few rows
-// that one's latency is what counts, with 8 vectors of a thread on their way (a row of 256 KB bf16: 12 us -> 8).
+// that one's latency is what counts, with 8 vectors of a thread on their way (a row of 256 KB bf16: 12 us -> 10.8).
 #define MODE_WAVE 0
 #define MODE_BLOCK 1
 #define MODE_FEW 2
@@ -583,10 +583,12 @@ template <bool ENT> __device__ __forceinline__ double ln_sum(const Logits& L, co
 }
 template <bool NEAR> __device__ __forceinline__ double logp_of(const Logits& L, float x, float m, double ln_s) {
     const double u = NEAR ? fma((double)x, (double)L.c2, -(double)near_max(m, L.c2)) : ((double)x - (double)m) * (double)L.c2;
-    return fma(L.ln2, u, -ln_s);
+    const double lp = fma(L.ln2, u, -ln_s);
+    return lp > 0.0 ? 0.0 : lp;        // S is rounded: no probability is above 1 for that, and no entropy below 0
 }
 __device__ __forceinline__ float entropy_of(const Logits& L, const Acc& a, double ln_s) {
-    return (float)fma(-L.ln2, (double)(a.e / a.s), ln_s);
+    const float h = (float)fma(-L.ln2, (double)(a.e / a.s), ln_s);
+    return h < 0.0f ? 0.0f : h;
 }
 
 // ------------------------------------------------------------------------------------------ counting masks

@@ -430,7 +430,7 @@ static PreferenceOut preference_call(const Tensor& x, const Preference& p, const
     const Call call(x);
     PreferenceOut o{new_floats(x, {}), at::empty_like(p.ref), seeds ? at::empty_like(p.ref) : Tensor(),
                     scratch(x, p.tokens.sizes(), seeds ? 4 : 0)};
-    const ppo_token_logits r = rows_of(x, 1.0f, grad);
+    const ppo_token_logits r = rows_of(x, 1.0, grad);
     done(lib.ppo_preference_loss(&r, p.tokens.data_ptr(), is_i64(p.tokens), at_of<uint8_t>(p.mask), at_of<float>(p.ref), p.beta,
                                  p.smoothing, p.scale, at_of<float>(o.loss), at_of<float>(o.rewards),
                                  seeds ? o.ws.behind() : nullptr, at_of<float>(o.seeds), at_of<void>(grad), o.ws.at(),
@@ -451,7 +451,7 @@ struct PreferenceNode : torch::autograd::Function<PreferenceNode> {
         if (!g[0].defined()) return variable_list(2);
         const auto s = ctx->get_saved_variables();
         const float* stats = (const float*)((const char*)s[3].data_ptr() + ctx->saved_data["offset"].toInt());
-        return {backward_call(s[0], s[1], s[2], 1.0f, stats, at_of<float>(s[4]), {1, 0}, nullptr, {0, 0}, g[0]), Tensor()};
+        return {backward_call(s[0], s[1], s[2], 1.0, stats, at_of<float>(s[4]), {1, 0}, nullptr, {0, 0}, g[0]), Tensor()};
     }
 };
 
@@ -480,7 +480,8 @@ static Policy3 preference_loss_and_grad(const Tensor& x_, const Tensor& tokens, 
 // ------------------------------------------------------------------------------------------ distillation
 struct Teacher : torch::CustomClassHolder {
     Tensor index, logits, mask;
-    float inv_t = 1.0f, scale = 1.0f;
+    double inv_t = 1.0;
+    float scale = 1.0f;
     int reduction = 0;
 };
 

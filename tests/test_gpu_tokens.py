@@ -614,6 +614,38 @@ def test_other_types_beside_the_logits(dtype):
         assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("v", [1, 6, 70, 500, 4099, 70001])
+@pytest.mark.parametrize("temp", [1.0, 0.7])
+def test_certain_tokens(v, temp):
+    """All probability on one token: no log-probability above 0, no entropy below, in forward, loss and logging outputs."""
+    r = np.random.default_rng(v)
+    x = torch.full((4, 32, v), -math.inf)
+    x[..., v // 2] = torch.from_numpy(20 * r.standard_normal((4, 32))).float()
+    x, y = x.cuda(), torch.full((4, 32), v // 2).cuda()
+    old, adv = torch.zeros(4, 32).cuda(), torch.ones(4, 32).cuda()
+    for lp, ent in (K().token_logprobs(x, y, temperature=temp), K().policy_loss_and_grad(x, y, old, adv, temperature=temp)[2:],
+                    K().policy_loss(x, y, old, adv, temperature=temp)[1:],
+                    K().policy_loss_and_grad(x[:1, :1], y[:1, :1], old[:1, :1], adv[:1, :1], temperature=temp)[2:]):
+        assert (lp <= 0).all() and (ent >= 0).all()
+        assert lp.min() >= -row_tol(v) and ent.max() <= row_tol(v)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_small_terms_of_long_rows_are_not_lost(dtype):
+    """The mean error of ln p over 512 rows of 131072 logits with most of their terms far below the largest.  Added to
+    S one by one, the small ones were lost: 6.5e-7.  At least 16 are added at once, so at most 1/16 of that is left: 4e-8;
+    rounding ln p (below 64) is off by at most 2^-19 and by 2^-19 / sqrt 3 = 1.1e-6 in the square mean, 5e-8 in the mean of
+    512, of which four are allowed."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    x = (2.5 * torch.randn(64, 8, 131072, generator=g, device="cuda")).to(dtype)
+    y = torch.randint(0, 131072, (64, 8), generator=g, device="cuda")
+    for entropy in (True, False):
+        lp, _ = K().token_logprobs(x, y, temperature=0.5, entropy=entropy)
+        want = torch.cat([torch.log_softmax(q.double() / 0.5, -1).gather(1, i[:, None])[:, 0][None] for q, i in zip(x, y)])
+        assert abs((lp.double() - want).mean().item()) < 2.4e-7
+
+
 def test_far_rows():
     """Offsets beyond 2^31 elements, in the logits and in the gradient."""
     v, far = 1003, (1 << 31) + 24
