@@ -1605,11 +1605,14 @@ static int weights_of(Weights* o, const uint8_t* mask, int reduction, float scal
     return 0;
 }
 
+// logprobs64, which are summed over a sequence and compared, are computed with E: what ln_sum takes back with it is up to
+// 1e-7 a token, the same way in all of them.
 static void launch_logprobs(Logits L, int dtype, const void* tokens, int i64, const uint8_t* mask, float* logprobs,
                             double* logprobs64, float* entropy, RowStats* stats, Acc* acc, hipStream_t st) {
+    const bool with_e = entropy || logprobs64;
     if (const int parts = acc ? split_parts(L, dtype, 64, 128 * 1024) : 0) {
         const Split sp = {acc, nullptr, parts};
-        BY_FLAG(entropy != nullptr, ENT, {
+        BY_FLAG(with_e, ENT, {
             BY_TYPE(dtype, T, (split_stats_kernel<T, ENT><<<dim3((unsigned)L.n, parts), 256, 0, st>>>(L, mask, tokens, i64, sp)))
             split_logprobs_kernel<ENT><<<(int)(L.n + 3) / 4, 256, 0, st>>>(L, mask, logprobs, logprobs64, entropy, stats, sp);
         })
@@ -1620,7 +1623,7 @@ static void launch_logprobs(Logits L, int dtype, const void* tokens, int i64, co
             L, tokens, i64, mask, logprobs, logprobs64, entropy, stats)))))
         return;
     }
-    BY_TYPE(dtype, T, BY_MODE(stream_mode(L, dtype), MODE, BY_FLAG(entropy != nullptr, ENT, BY_FLAG(stats != nullptr, KEEP, {
+    BY_TYPE(dtype, T, BY_MODE(stream_mode(L, dtype), MODE, BY_FLAG(with_e, ENT, BY_FLAG(stats != nullptr, KEEP, {
         EACH_LAUNCH(L, MODE == MODE_WAVE, grid, (logprobs_kernel<T, MODE, ENT, KEEP><<<grid, stream_threads(L, dtype, MODE), 0, st>>>(
             L, tokens, i64, mask, logprobs, logprobs64, entropy, stats)))
     }))))

@@ -415,6 +415,20 @@ def test_preference_loss(b, t, v, dtype, beta, smoothing):
     close_grad(torch.autograd.grad(out[0], x)[0], grad, size, v, 2 * tol)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t,v", [(511, 50001), (2, 131072), (700, 900)])
+def test_rewards_of_long_sequences(t, v, dtype):
+    """A reward is a difference of sums of many log-probabilities, where a systematic error of theirs adds up: half a step
+    of S (2^-24) is allowed for it, beside four times the spread of t independent errors of a step (2^-23)."""
+    x, y, m = make(31, 4, t, v, dtype, masked=False)
+    each = torch.stack([torch.log_softmax(q.double(), -1).gather(1, i[:, None])[:, 0] for q, i in zip(x, y)])
+    ref = each.sum(1).float()
+    want = each.sum(1) - ref.double()
+    tol = t * 2.0 ** -24 + 4 * math.sqrt(t) * 2.0 ** -23
+    for rewards in (K().preference_loss(x, y, ref, m, beta=1.0)[1], K().preference_loss_and_grad(x, y, ref, m, beta=1.0)[2]):
+        close(rewards, f64(want), tol + 2.0 ** -24 * np.abs(f64(want)))
+
+
 def test_preference_far_apart():
     """Rewards so far apart that a sigmoid is 0 or 1, and an impossible token."""
     x, y, _ = make(3, 4, 3, 90, torch.float32, masked=False)
