@@ -799,6 +799,27 @@ def test_a_training_step_with_all_of_them():
     assert (torch.autograd.grad(logits, w, total)[0].cpu() - grad).abs().max() < 1e-5 * grad.abs().max()
 
 
+def test_the_gradient_takes_the_logits_place():
+    """A model's step as the documentation shows it: the loss's gradient over the logits, a view, and backward from there."""
+    torch.manual_seed(1)
+    ids, mask = torch.randint(0, 901, (3, 9)).cuda(), torch.rand(3, 8).cuda() < 0.8
+    model = torch.nn.Sequential(torch.nn.Embedding(901, 32), torch.nn.Tanh(), torch.nn.Linear(32, 901)).cuda()
+    advantages = torch.randn(3, device="cuda")
+    grads = []
+    for in_place in (False, True):
+        model.zero_grad()
+        logits = model(ids)[:, :-1]
+        with torch.no_grad():
+            old = K().token_logprobs(logits, ids[:, 1:], mask)[0] - 0.05
+        if in_place:
+            logits.backward(K().policy_loss_and_grad(logits, ids[:, 1:], old, advantages, mask, out=logits.detach())[1])
+        else:
+            K().policy_loss(logits, ids[:, 1:], old, advantages, mask)[0].backward()
+        grads.append([p.grad.clone() for p in model.parameters()])
+    for a, b in zip(*grads):   # two forms of the same arithmetic: 2^-20 of the largest entry
+        assert a.abs().max() > 0 and (a - b).abs().max() <= 2.0 ** -20 * a.abs().max()
+
+
 @pytest.mark.parametrize("v", [6, 900])
 def test_gradients_are_the_differences_of_the_losses(v):
     x, y, m = make(30, 2, 3, v, torch.float32)
