@@ -282,7 +282,10 @@ __device__ __forceinline__ Acc stream_stats(const T* body, int nvec, float edge,
             fetch();
             __builtin_amdgcn_sched_barrier(0);    // the loads stay ahead of the arithmetic
 #pragma unroll
-            for (int k = 0; k < DEPTH; k += M) acc_vecs<T, M, ENT, NEAR>(a, v + k, c2);
+            for (int k = 0; k < DEPTH; k += M) {
+                acc_vecs<T, M, ENT, NEAR>(a, v + k, c2);
+                if (DEPTH > M) __builtin_amdgcn_sched_barrier(0);    // two groups unpacked at once would not fit the registers
+            }
         }
         if (steps > 0) {
 #pragma unroll
@@ -294,7 +297,10 @@ __device__ __forceinline__ Acc stream_stats(const T* body, int nvec, float edge,
         __builtin_amdgcn_sched_barrier(0);
         if (steps > 0) {
 #pragma unroll
-            for (int k = 0; k < DEPTH; k += M) acc_vecs<T, M, ENT, NEAR>(a, v + k, c2);
+            for (int k = 0; k < DEPTH; k += M) {
+                acc_vecs<T, M, ENT, NEAR>(a, v + k, c2);
+                if (DEPTH > M) __builtin_amdgcn_sched_barrier(0);    // two groups unpacked at once would not fit the registers
+            }
         }
 #pragma unroll
         for (int k = 0; k < DEPTH; ++k)
