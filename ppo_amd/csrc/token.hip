@@ -530,21 +530,46 @@ struct Weights {              // how much a row counts
 };
 
 #define COUNT_HERE 4096       // rows up to which that is cheaper than a launch (16 bytes of the mask are one load)
+#define COUNT_SEQS 64         // and, for means over sequences, as many as a wave has lanes
 
-// This thread's part of the counted rows.
-__device__ __forceinline__ float count_mask(const Weights& w, int64_t n, const Part& p) {
+// How many of 16 bytes, the first `skip` left out, are not 0.
+__device__ __forceinline__ int count_16(const uint8_t* at, int skip) {
+    u32x4 v;
+    __builtin_memcpy(&v, at, 16);
     int k = 0;
-    if (w.count_here) {
-        const int whole = (int)n / 16;
-        for (int j = p.tid; j < whole; j += p.nt) {
-            u32x4 v;
-            __builtin_memcpy(&v, w.mask + 16 * j, 16);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)   // bytes that are not 0
-                k += __popc((((v[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | v[i]) & 0x80808080u);
-        }
+    for (int i = 0; i < 4; ++i) {
+        const int out = min(max(skip - 4 * i, 0), 4) * 8;
+        k += __popc((((v[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | v[i]) & (uint32_t)(0x80808080ull << out));
+    }
+    return k;
+}
+
+// This thread's part of the counted rows; for means over sequences, of 128 times those of sequence b and of the
+// sequences that have one: g lanes of a wave take a sequence.
+__device__ __forceinline__ float count_mask(const Weights& w, int64_t n, int64_t n_tok, uint32_t b, const Part& p) {
+    int k = 0;
+    if (w.count_here && w.reduction == RED_TOKEN) {
+        const int whole = (int)n / 16;
+        for (int j = p.tid; j < whole; j += p.nt) k += count_16(w.mask + 16 * j, 0);
         const int j = whole * 16 + p.tid;
         if (p.tid < 16 && j < (int)n) k += w.mask[j] != 0;
+    } else if (w.count_here) {
+        int sh = 6;
+        while (((int)w.n_seq << sh) > p.nt) --sh;
+        const int g = 1 << sh, mine = p.tid >> sh, lane = p.tid & (g - 1), t = (int)n_tok;
+        if (p.first < ((int)w.n_seq << sh)) {     // some lane of this wave has a part
+            const uint8_t* mask = w.mask + (mine < (int)w.n_seq ? mine : 0) * t;
+            if (t < 16) {
+                for (int c = lane; c < t; c += g) k += mask[c] != 0;
+            } else {          // the last 16 bytes overlap the ones before
+                for (int c = lane * 16; c < t; c += g * 16) k += count_16(mask + min(c, t - 16), max(c + 16 - t, 0));
+            }
+            if (mine >= (int)w.n_seq) k = 0;
+            const uint64_t lanes = (g == 64 ? ~0ull : (1ull << g) - 1) << (threadIdx.x & 63 & ~(g - 1));
+            const bool some = __ballot(k > 0) & lanes;
+            k = (mine == (int)b ? 128 * k : 0) + (some && lane == 0);
+        }
     }
     return (float)k;          // below 2^24 in any sum: exact
 }
@@ -553,7 +578,9 @@ __device__ __forceinline__ float row_weight(const Weights& w, const Place& at, i
     float d = 1.0f;           // rows are fewer than 2^30: rounded once by 2^-24 at most, as the quotient is
     if (w.reduction != RED_SUM && !w.mask) d = (float)(w.n_seq * n_tok);
     else if (w.reduction == RED_TOKEN) d = w.count_here ? counted : (float)w.totals[0];
-    else if (w.reduction == RED_SEQ) d = (float)((int64_t)w.seq_len[at.b] * (int64_t)w.totals[1]);
+    else if (w.reduction == RED_SEQ)
+        d = w.count_here ? (float)(((int)counted >> 7) * ((int)counted & 127))
+                         : (float)((int64_t)w.seq_len[at.b] * (int64_t)w.totals[1]);
     return w.scale / d;
 }
 
@@ -847,7 +874,7 @@ __global__ __launch_bounds__(1024, 4) void policy_forward_kernel(Logits L, Polic
             const T* x = row_in<T>(L, at);
             const PolicyIn in = policy_in(L, p, x, r, at);
             Acc a;
-            if (!stream_row<T, MODE, true, true>(x, L.V, L.c2, count_mask(p.w, L.n, part_of<WAVE>()), lds, a)) return;
+            if (!stream_row<T, MODE, true, true>(x, L.V, L.c2, count_mask(p.w, L.n, L.n_tok, at.b, part_of<WAVE>()), lds, a)) return;
             d = policy_done<false>(L, p, in, a, at, a.n);
             st = {a.m, a.s, d.h, 0.0f};
         }
@@ -887,7 +914,7 @@ __global__ __launch_bounds__(1024, 4) void policy_kernel(Logits L, PolicyArgs p)
             Row<T, CH> row;
             const PolicyIn in = policy_in(L, p, x, r, at);
             row_load(row, x, s, q);
-            const float counted = count_mask(p.w, L.n, q);
+            const float counted = count_mask(p.w, L.n, L.n_tok, at.b, q);
             asm volatile("" :: "v"(in.xt));   // read before the barrier: the gradient may overwrite it
             Acc a = row_stats<T, CH, WAVE, true>(row, x, s, q, L.c2, counted);
             RowGrad g;
@@ -1134,7 +1161,7 @@ __global__ __launch_bounds__(256) void policy_split_kernel(Logits L, PolicyArgs 
             in.ref = p.ref ? p.ref[r] : 0.0f;
             in.xt = sp.acc[r * sp.parts].n;
             const Acc a = split_join<true>(sp, r, L.c2);
-            d = policy_done<false>(L, p, in, a, at, wave_sum(count_mask(p.w, L.n, part_of<true>())));
+            d = policy_done<false>(L, p, in, a, at, wave_sum(count_mask(p.w, L.n, L.n_tok, at.b, part_of<true>())));
             if (threadIdx.x == 0) sh.grad = policy_seed(L, d, a.m, a.s, in.tok);
         }
         __syncthreads();
@@ -1299,7 +1326,7 @@ __global__ __launch_bounds__(1024, 4) void distill_forward_kernel(Logits L, Teac
         float ent = 0.0f;
         if (threadIdx.x < 64) ent = teacher_load(p, L, r, x, teach);
         Acc a;
-        if (!stream_row<T, MODE, false, true>(x, L.V, L.c2, count_mask(p.w, L.n, part_of<false>()), lds, a)) return;
+        if (!stream_row<T, MODE, false, true>(x, L.V, L.c2, count_mask(p.w, L.n, L.n_tok, at.b, part_of<false>()), lds, a)) return;
         loss = teacher_loss(p, teach, ent, a, L) / (L.c * L.c);
         st.m = a.m;
         st.s = a.s;
@@ -1330,7 +1357,7 @@ __global__ __launch_bounds__(1024, 4) void distill_kernel(Logits L, TeacherArgs 
         row_load(row, x, s, q);
         float ent = 0.0f;
         if (q.first == 0) ent = teacher_load(p, L, r, x, teach);
-        Acc a = row_stats<T, CH, false, false>(row, x, s, q, L.c2, count_mask(p.w, L.n, q));
+        Acc a = row_stats<T, CH, false, false>(row, x, s, q, L.c2, count_mask(p.w, L.n, L.n_tok, at.b, q));
         if ((threadIdx.x & 63) == 0) sh.acc[threadIdx.x >> 6] = a;
         __syncthreads();
         a = acc_waves<false, true>(sh.acc, L.c2);
@@ -1396,7 +1423,7 @@ template <typename T> __global__ __launch_bounds__(256) void distill_split_kerne
         for (int k = threadIdx.x; k < 2 + 3 * p.K; k += 256) entries[k] = from[k < 2 ? k : k + 2];
         if (q.first == 0) {
             Acc a = split_join<false>(sp, r, L.c2);
-            a.n = wave_sum(count_mask(p.w, L.n, part_of<true>()));
+            a.n = wave_sum(count_mask(p.w, L.n, L.n_tok, at.b, part_of<true>()));
             if (threadIdx.x == 0) joined = a;
         }
         __syncthreads();
@@ -1606,7 +1633,8 @@ static void count_rows(const Weights& o, const ppo_token_logits* x, const Worksp
 static int weights_of(Weights* o, const uint8_t* mask, int reduction, float scale, const ppo_token_logits* x,
                       const Workspace& w) {
     if (reduction != RED_SUM && reduction != RED_TOKEN && reduction != RED_SEQ) return PPO_E_BADARG;
-    const int here = mask && reduction == RED_TOKEN && x->n_seq * x->n_tok <= COUNT_HERE;
+    const int here = mask && reduction != RED_SUM && x->n_seq * x->n_tok <= COUNT_HERE &&
+                     (reduction == RED_TOKEN || x->n_seq <= COUNT_SEQS);
     *o = {mask, w.seq_len, w.totals, reduction, here, scale, x->n_seq};
     return 0;
 }

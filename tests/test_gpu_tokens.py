@@ -342,6 +342,33 @@ def test_policy_advantages_of_other_layouts(shape):
     assert torch.equal(K().policy_loss_and_grad(x, y, old_t, adv_t, m.to(torch.uint8))[1], got[1])
 
 
+SEQS = [(1, 1), (1, 16), (1, 4000), (2, 1), (2, 15), (2, 17), (3, 33), (5, 64), (6, 255), (8, 500), (33, 7), (63, 65), (64, 16), (64, 64),
+        (65, 3)]
+
+
+@pytest.mark.parametrize("b,t,v", [(b, t, v) for v in (300, 2600, 21000) for b, t in SEQS if b * t * v < 3e7])
+def test_means_over_sequences(b, t, v):
+    """Every counted row's weight is 1 / (counted rows of its sequence * sequences with one): the gradient of the loss with
+    respect to a row's log-probability, found at the token of a row of equal logits, where it is weight * (1 - 1/v)."""
+    r = np.random.default_rng(b * 1000 + t)
+    mask = r.random((b, t)) < r.choice([0.02, 0.5, 0.97], (b, 1))
+    mask[0, -1] = True
+    n = mask.sum(1)
+    want = mask / np.maximum(n, 1)[:, None] / (n > 0).sum()
+    x, m = torch.zeros(b, t, v, device="cuda"), torch.from_numpy(mask).cuda()
+    y = torch.from_numpy(r.integers(0, v, (b, t))).cuda()
+    one = torch.ones(b, t, device="cuda")
+    old = one * -math.log(v)
+    leaf = x.clone().requires_grad_(True)
+    for sign, grad in ((-1, K().policy_loss_and_grad(x, y, old, one, m, reduction="sequence_mean")[1]),
+                       (-1, torch.autograd.grad(K().policy_loss(leaf, y, old, one, m, reduction="sequence_mean")[0], leaf)[0]),
+                       (-1, K().distillation_loss_and_grad(x, y[..., None], one[..., None], m, reduction="sequence_mean")[1]),
+                       (-1, torch.autograd.grad(K().distillation_loss(leaf, y[..., None], one[..., None], m,
+                                                                      reduction="sequence_mean")[0], leaf)[0])):
+        got = sign * torch.take_along_dim(grad, y[..., None], 2)[..., 0] / (1 - 1 / v)
+        close(got, want, want * (3 * row_tol(v) + 2.0 ** -20))
+
+
 def test_many_rows_and_many_sequences():
     """More rows than workgroups, and masks counted in two launches."""
     for b, t, v in [(5000, 9, 33), (40000, 1, 5), (2, 20000, 9)]:
