@@ -964,26 +964,27 @@ __global__ __launch_bounds__(1024, 4) void policy_kernel(Logits L, PolicyArgs p)
     row_loss<WAVE>(p, r, L.n, weighted_loss(p, d.o, d.h));
 }
 
-// Rows of at most 256 logits, as of a head of a few actions: G lanes a row (4 up to 64 logits, 16 beyond), 16 logits a lane
-// at most, element by element.  A wave's fp64 arithmetic then serves 64 / G rows: 524288 rows of 6 logits with their
-// gradient took 413 us with a wave each.
+// Rows of at most 256 logits: G lanes a row, at most 16 logits a lane (8 of a lane that has a row, as of a head of a few
+// actions, by itself), element by element.  A wave's fp64 arithmetic then serves 64 / G rows: 524288 rows of 6 logits
+// with their gradient take 21 us with a lane each, 36 with four and took 413 with a wave.
 template <typename T, int G> struct Tiny {
-    float f[16];
+    static constexpr int PER = G == 1 ? 8 : 16;
+    float f[PER];
     int lane;
 
     __device__ __forceinline__ Acc load(const T* x, int V, float c2) {
         lane = threadIdx.x & (G - 1);
         Acc a = acc_empty();
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
+        for (int k = 0; k < PER; ++k) {
             f[k] = -__builtin_inff();
             if (k * G + lane < V) f[k] = wide(x[k * G + lane]);
         }
 #pragma unroll
-        for (int k = 0; k < 16; ++k) a.m = fmaxf(a.m, f[k]);
+        for (int k = 0; k < PER; ++k) a.m = fmaxf(a.m, f[k]);
         a.m = group(a.m, [](float p, float q) { return fmaxf(p, q); });
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
+        for (int k = 0; k < PER; ++k)
             if (k * G < V) acc_add<true>(a, f[k], c2);
         a.s = group(a.s, [](float p, float q) { return p + q; });
         a.e = group(a.e, [](float p, float q) { return p + q; });
@@ -995,12 +996,13 @@ template <typename T, int G> struct Tiny {
             v = op(v, ror<0x128>(v));
             v = op(v, ror<0x124>(v));
         }
+        if (G == 1) return v;
         v = op(v, ror<0x4e>(v));   // quads: lanes 2, 3, 0, 1
         return op(v, ror<0xb1>(v));   // lanes 1, 0, 3, 2
     }
     __device__ __forceinline__ void store(T* out, int V, float c2, const RowGrad& g) const {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
+        for (int k = 0; k < PER; ++k) {
             const int i = k * G + lane;
             if (i < V) {
                 const float d = grad_of<true, false>(g, f[k], c2);
@@ -1552,10 +1554,13 @@ static Logits logits_of(const ppo_token_logits* x, void* grad) {
 
 static int64_t row_bytes(const Logits& L, int dtype) { return (int64_t)L.V * (dtype == PPO_F32 ? 4 : 2); }
 
-// Lanes of a row of so few logits that several share a wave; 0: more than that.
-static int tiny_lanes(const Logits& L) { return L.V <= 64 ? 4 : L.V <= 256 ? 16 : 0; }
+// Lanes of a row of so few logits that several share a wave; 0: more than that.  One lane's accesses are as far apart as
+// the rows: 524288 rows, log-probabilities and loss with gradient, in us with one lane / with four: of 6 logits 7 / 18 and
+// 21 / 36, of 8 12 / 17 and 30 / 34, of 12 10 / 18 and 40 / 35, of 16 20 / 17 and 64 / 36.
+static int tiny_lanes(const Logits& L) { return L.V <= 8 ? 1 : L.V <= 64 ? 4 : L.V <= 256 ? 16 : 0; }
 #define BY_LANES(lanes, G, ...)                                                    \
-    if ((lanes) == 4) { constexpr int G = 4; __VA_ARGS__; }                        \
+    if ((lanes) == 1) { constexpr int G = 1; __VA_ARGS__; }                        \
+    else if ((lanes) == 4) { constexpr int G = 4; __VA_ARGS__; }                   \
     else { constexpr int G = 16; __VA_ARGS__; }
 
 // A wave takes a row of up to 4 KB by itself: its 64 lanes hold that in four vectors each.

@@ -323,6 +323,32 @@ def test_policy_loss(reduction, b, t, v, dtype, kl, ent):
         close(K().policy_loss(x, y, old_t, adv_t, m, **more)[0], loss, tol, "loss")
 
 
+EDGES = [8, 9, 16, 17, 63, 65, 256, 257, 1023, 1024, 1025, 2047, 2048, 2049, 8192, 24575, 24576, 24577, 49151, 49152, 49153, 65535, 65536, 65537]
+
+
+@pytest.mark.parametrize("v", EDGES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sizes_at_which_the_form_changes(v, dtype):
+    """On both sides of each size at which rows are worked on in another way, 130 rows and 3: log-probabilities, entropy and the
+    gradient of a policy loss that has all terms, from both forms of it."""
+    for b, t in ((10, 13), (1, 3)):
+        x, y, m = make(v + t, b, t, v, dtype)
+        fx, fy, fm, old, adv, ref, old_t, adv_t, ref_t = policy_inputs(v, x, y, m, 1.0)
+        w = O.weights(fm, b, t, "token_mean", 64.0)
+        loss, grad, size, _ = O.policy(fx, fy, old, adv, fm, ref, w, 0.2, 0.2, 0.05, 0.02, 1.0)
+        lp, h = O.logprobs(fx, fy, fm, 1.0)
+        more = dict(ref_logprobs=ref_t, kl_coef=0.05, entropy_coef=0.02, scale=64.0)
+        off = 4 * float(logp_tol(lp, v).max()) + 2.0 ** -21
+        tol = mean_tol(w, (np.abs(adv) * 2 + 0.5 + 0.02 * (1 + h)) * off) + 2.0 ** -23 * abs(loss) + 1e-12
+        got = K().policy_loss_and_grad(x, y, old_t, adv_t, m, **more)
+        out = K().policy_loss(x.requires_grad_(True), y, old_t, adv_t, m, **more)
+        for some in (got, (out[0], torch.autograd.grad(out[0], x)[0], out[1], out[2])):
+            close(some[0], loss, tol, "loss")
+            close_grad(some[1], grad, size, v, off)
+            close(some[2].reshape(-1), lp, logp_tol(lp, v))
+            close(some[3].reshape(-1), h, 2 * row_tol(v) * (1 + np.abs(h)) + 1e-6)
+
+
 @pytest.mark.parametrize("shape", ["column", "vector", "expanded", "transposed", "half"])
 def test_policy_advantages_of_other_layouts(shape):
     b, t, v = 3, 4, 301
