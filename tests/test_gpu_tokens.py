@@ -762,6 +762,33 @@ def test_same_bits_every_time_and_on_another_stream():
                 assert torch.equal(p, q) and torch.equal(p, r)
 
 
+def test_two_threads_at_once():
+    """Calls from two threads, each on a stream of its own, whose workspaces and host code run at the same time."""
+    import threading
+    sets = [make(40 + k, 4, 40, v, dtype) for k, (v, dtype) in enumerate([(33000, torch.bfloat16), (140001, torch.float16)])]
+    wants = [all_three(*s) for s in sets]
+    torch.cuda.synchronize()
+    gots = [[], []]
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                gots[k].append(all_three(*sets[k]))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for want, got in zip(wants, gots):
+        assert len(got) == 10
+        for one in got:
+            for a, b in zip(want, one):
+                for p, q in zip(a, b):
+                    assert torch.equal(p, q)
+
+
 def test_captured_graphs():
     """Each form captured and replayed with new inputs, eager work between; two graphs replayed on two streams."""
     v = 3001
