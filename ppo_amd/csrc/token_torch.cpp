@@ -65,6 +65,7 @@ static at::IntArrayRef check_logits(const Tensor& x) {
                       "logits must be a tensor [sequences, tokens, vocabulary] or [tokens, vocabulary]");
     TORCH_CHECK_VALUE(type_code(x.scalar_type()) >= 0, "logits of type ", type_name(x.scalar_type()),
                       ": float32, bfloat16 and float16 are supported");
+    TORCH_CHECK_VALUE(!x.is_neg(), "logits that torch has yet to negate (a lazy view): resolve_neg() them first");
     TORCH_CHECK_VALUE(x.size(-1) > 0, "logits over an empty vocabulary");
     TORCH_CHECK_VALUE(x.size(-1) == 1 || x.stride(-1) == 1, "the vocabulary must be the contiguous dimension of the logits");
     return x.sizes().slice(0, x.dim() - 1);
@@ -103,9 +104,11 @@ static Tensor mask_of(const Tensor& x, const OptTensor& t, at::IntArrayRef shape
     check(x, *t, "mask", Kind::MASK, shape);
     return t->contiguous();
 }
+// The numbers themselves, where complex arithmetic has left a view that torch has yet to negate.
+static Tensor resolved(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 static Tensor floats(const Tensor& x, const Tensor& t, const char* name, at::IntArrayRef shape) {
     check(x, t, name, Kind::FLOATS, shape);
-    return t.scalar_type() == at::kFloat ? t : t.to(at::kFloat);
+    return resolved(t.scalar_type() == at::kFloat ? t : t.to(at::kFloat));
 }
 
 static double inverse(double temperature) {
@@ -133,6 +136,7 @@ static std::pair<uintptr_t, uintptr_t> span(const Tensor& t) {
 static Tensor check_out(const Tensor& out, const Tensor& x, std::initializer_list<std::pair<const char*, Tensor>> others) {
     TORCH_CHECK_VALUE(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type() && out.device() == x.device(),
                       "out must have the shape, the type and the device of the logits");
+    TORCH_CHECK_VALUE(!out.is_neg(), "out is a view that torch has yet to negate");
     TORCH_CHECK_VALUE(out.size(-1) == 1 || out.stride(-1) == 1, "the vocabulary must be the contiguous dimension of out");
     int64_t reach = out.size(-1);
     for (int64_t d = out.dim() - 2; d >= 0; --d) {
@@ -262,7 +266,7 @@ struct LogprobsNode : torch::autograd::Function<LogprobsNode> {
         return {lp};
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
-        const Tensor g_lp = g[0], g_ent = g.size() > 1 ? g[1] : Tensor();
+        const Tensor g_lp = resolved(g[0]), g_ent = g.size() > 1 ? resolved(g[1]) : Tensor();
         if (!g_lp.defined() && !g_ent.defined()) return variable_list(2);
         const auto s = ctx->get_saved_variables();
         const Strides none{0, 0};
@@ -358,7 +362,7 @@ struct PolicyNode : torch::autograd::Function<PolicyNode> {
         const float* g_lp = stats + 4 * tokens.numel();
         const Strides dense = row_strides(tokens);
         return {backward_call(x, tokens, s[2], ctx->saved_data["inv_t"].toDouble(), stats, g_lp, dense,
-                              ctx->saved_data["entropy"].toBool() ? g_lp + tokens.numel() : nullptr, dense, g[0]),
+                              ctx->saved_data["entropy"].toBool() ? g_lp + tokens.numel() : nullptr, dense, resolved(g[0])),
                 Tensor()};
     }
 };
@@ -451,7 +455,7 @@ struct PreferenceNode : torch::autograd::Function<PreferenceNode> {
         if (!g[0].defined()) return variable_list(2);
         const auto s = ctx->get_saved_variables();
         const float* stats = (const float*)((const char*)s[3].data_ptr() + ctx->saved_data["offset"].toInt());
-        return {backward_call(s[0], s[1], s[2], 1.0, stats, at_of<float>(s[4]), {1, 0}, nullptr, {0, 0}, g[0]), Tensor()};
+        return {backward_call(s[0], s[1], s[2], 1.0, stats, at_of<float>(s[4]), {1, 0}, nullptr, {0, 0}, resolved(g[0])), Tensor()};
     }
 };
 
@@ -495,7 +499,7 @@ static c10::intrusive_ptr<Teacher> teacher_args(const Tensor& x, const Tensor& i
     full.push_back(index.size(-1));
     p->index = integers(x, index, "teacher_tokens", full);
     check(x, values, "teacher_logits", Kind::LOGITS, full);
-    p->logits = values.contiguous();
+    p->logits = resolved(values).contiguous();
     p->mask = mask_of(x, mask, shape);
     p->inv_t = inverse(temperature);
     p->reduction = reduction;
@@ -536,10 +540,10 @@ struct TeacherNode : torch::autograd::Function<TeacherNode> {
         const Tensor &x = s[0], &index = s[1], &values = s[2];
         const float* stats = (const float*)((const char*)s[4].data_ptr() + ctx->saved_data["offset"].toInt());
         const Call call(x);
-        const Tensor grad = grad_like(x);
+        const Tensor factor = resolved(g[0]), grad = grad_like(x);
         const ppo_token_logits r = rows_of(x, ctx->saved_data["inv_t"].toDouble(), grad);
         done(lib.ppo_distillation_backward(&r, index.data_ptr(), is_i64(index), values.data_ptr(), type_code(values.scalar_type()),
-                                           (int)index.size(-1), at_of<uint8_t>(s[3]), stats, at_of<float>(g[0]), grad.data_ptr(),
+                                           (int)index.size(-1), at_of<uint8_t>(s[3]), stats, at_of<float>(factor), grad.data_ptr(),
                                            call.stream));
         return {once(grad), Tensor()};
     }
