@@ -405,8 +405,8 @@ int ppo_preference_loss(const ppo_token_logits* x, const void* tokens, int token
  * [rows, top] of a type of their own): q = softmax(teacher_logits * inv_temperature) over the entries whose
  * token is not negative (others are padding), p the student's softmax over the whole vocabulary,
  *   token_losses[r] = temperature^2 * sum_k q_k (ln q_k - ln p[token_k]),  loss = sum of weight * token_losses
- * A row without entries has loss and gradient 0; a token that appears twice counts with both entries; a
- * token >= vocab makes the row NaN.  top <= PPO_MAX_TEACHER_TOP.  grad != NULL: dloss/dlogits in the same
+ * A row without entries has loss and gradient 0 whatever its logits are; a token that appears twice counts
+ * with both entries; a token >= vocab makes the row NaN.  top <= PPO_MAX_TEACHER_TOP.  grad != NULL: dloss/dlogits in the same
  * pass; otherwise, with row_stats, ppo_distillation_backward computes it (times *grad_factor) later. */
 int ppo_distillation_loss(const ppo_token_logits* x, const void* teacher_tokens, int tokens_are_i64,
                           const void* teacher_logits, int teacher_dtype, int top, const uint8_t* mask,

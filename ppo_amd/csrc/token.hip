@@ -1287,11 +1287,12 @@ __device__ __forceinline__ float teacher_loss(const TeacherArgs& p, const Teache
     return *s.bad ? __builtin_nanf("") : (float)((double)ent - cross);
 }
 
-// dL/dx_i = g (p_i - sum of the teacher's q at i): the bulk first, the K places after a barrier.  A teacher that gave
-// nothing teaches nothing.
+// dL/dx_i = g (p_i - sum of the teacher's q at i): the bulk first, the K places after a barrier.
 __device__ __forceinline__ RowGrad teacher_seed(const Teacher& s, float m, float sum, float g) {
-    return {m, *s.bad ? __builtin_nanf("") : *s.some ? g / sum : 0.0f, 0.0f, 0.0f, -1};
+    return {m, *s.bad ? __builtin_nanf("") : g / sum, 0.0f, 0.0f, -1};
 }
+// A teacher that gave padding only teaches nothing: zeros, whatever the logits are (0 times a NaN is none).
+__device__ __forceinline__ bool teaches(const Teacher& s) { return *s.bad || *s.some; }
 
 template <typename T, bool NEAR>
 __device__ __forceinline__ void teacher_places(const TeacherArgs& p, const Teacher& s, T* out, const Logits& L,
@@ -1365,7 +1366,9 @@ __global__ __launch_bounds__(1024, 4) void distill_kernel(Logits L, TeacherArgs 
         a = acc_waves<false, true>(sh.acc, L.c2);
         w = row_weight(p.w, at, L.n_tok, a.n);
         const float scale = w / L.c;
-        if (is_near(a.m, L.c2)) {
+        if (!teaches(teach)) {
+            row_fill(out, L.V, q, 0, 1, L.past);
+        } else if (is_near(a.m, L.c2)) {
             const RowGrad g = teacher_seed(teach, near_max(a.m, L.c2), a.s, scale);
             row_grad<T, CH, false, false>(row, x, out, s, q, L.c2, g, L.past);
             teacher_places<T, true>(p, teach, out, L, g, scale, s);
@@ -1432,9 +1435,13 @@ template <typename T> __global__ __launch_bounds__(256) void distill_split_kerne
         const Acc a = joined;
         w = row_weight(p.w, at, L.n_tok, a.n);
         const T* x = row_in<T>(L, at);
-        const RowGrad g = teacher_seed(teach, a.m, a.s, w / L.c);
-        row_map<T, false>(x, out, L.V, q, blockIdx.y, gridDim.y, L.c2, g, L.past);
-        teacher_places<T, false>(p, teach, out, L, g, w / L.c, Span<T>(x, L.V, out), blockIdx.y, gridDim.y);
+        if (teaches(teach)) {
+            const RowGrad g = teacher_seed(teach, a.m, a.s, w / L.c);
+            row_map<T, false>(x, out, L.V, q, blockIdx.y, gridDim.y, L.c2, g, L.past);
+            teacher_places<T, false>(p, teach, out, L, g, w / L.c, Span<T>(x, L.V, out), blockIdx.y, gridDim.y);
+        } else {
+            row_fill(out, L.V, q, blockIdx.y, gridDim.y, L.past);
+        }
         if (q.first == 0) loss = teacher_loss(p, teach, __int_as_float(from[2]), a, L) / (L.c * L.c);
     } else {
         row_fill(out, L.V, q, blockIdx.y, gridDim.y, L.past);
@@ -1459,6 +1466,10 @@ template <typename T> __global__ __launch_bounds__(1024) void distill_backward_k
     const T* x = row_in<T>(L, at);
     if (q.first == 0) teacher_load(p, L, r, x, teach);
     __syncthreads();
+    if (!teaches(teach)) {
+        row_fill(out, L.V, q, 0, 1, L.past);
+        return;
+    }
     const RowStats st = p.stats[r];
     const float g = (p.factor ? *p.factor : 1.0f) * st.w / L.c;
     const RowGrad rg = teacher_seed(teach, st.m, st.s, g);

@@ -1,10 +1,44 @@
 """GPU tests of the losses over a large vocabulary: layouts and inputs at the edges of what their documentation allows."""
+import math
+
 import pytest
 import torch
 
-from test_gpu_tokens import K, make
+from test_gpu_tokens import K, TYPES, make
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,t,v", [(3, 4, 70), (2, 300, 1003), (2, 5, 33000), (1, 3, 70001), (2, 2, 140001), (3, 30, 140001)])
+def test_a_row_without_entries_has_no_gradient_whatever_its_logits(b, t, v, dtype):
+    """Rows whose teacher gave padding only: loss and gradient are 0 though the logits are NaN or infinite, in each form,
+    and the other rows are as they are beside ordinary logits."""
+    x, y, _ = make(v + t, b, t, v, dtype, masked=False)
+    index = torch.stack([y, (y + 1) % v, y * 0 - 1], -1)
+    values = torch.stack([y * 0.0, y * 0.0 - 1, y * 0.0 + 9], -1)
+    none = torch.zeros(b, t, dtype=torch.bool, device="cuda")
+    none[0, 0] = none[-1, -1] = True
+    index[none] = -1
+    bad = x.clone()
+    bad[0, 0, v // 3] = math.nan
+    bad[-1, -1] = -math.inf
+    bad[-1, -1, v // 2] = math.inf
+    results = []
+    for logits in (x, bad):
+        both = K().distillation_loss_and_grad(logits, index, values)
+        place = logits.clone()
+        over = K().distillation_loss_and_grad(place, index, values, out=place)
+        leaf = logits.clone().requires_grad_(True)
+        loss, each = K().distillation_loss(leaf, index, values)
+        later = torch.autograd.grad(loss, leaf)[0]
+        results.append([*both, *over, loss.detach(), each, later])
+        for grad in (both[1], over[1], later):
+            assert (grad[none] == 0).all()
+        for each in (both[2], over[2], each):
+            assert (each[none] == 0).all() and torch.isfinite(each).all()
+    for a, c in zip(*results):
+        assert torch.equal(a, c)
 
 
 def negated(t):
