@@ -60,7 +60,13 @@ static int type_code(at::ScalarType t) {
     return t == at::kFloat ? PPO_F32 : t == at::kBFloat16 ? PPO_BF16 : t == at::kHalf ? PPO_F16 : -1;
 }
 
+// Outputs carry no forward-mode derivative, and one that is missing would be taken for zero.
+static void no_tangent(const Tensor& t, const char* name) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name, ": the losses over a vocabulary have no forward-mode derivative");
+}
+
 static at::IntArrayRef check_logits(const Tensor& x) {
+    no_tangent(x, "logits");
     TORCH_CHECK_VALUE(x.dim() == 2 || x.dim() == 3,
                       "logits must be a tensor [sequences, tokens, vocabulary] or [tokens, vocabulary]");
     TORCH_CHECK_VALUE(type_code(x.scalar_type()) >= 0, "logits of type ", type_name(x.scalar_type()),
@@ -76,6 +82,7 @@ enum class Kind { INTEGERS, MASK, FLOATS, LOGITS };
 // A tensor beside the logits: of its types, of this shape, where the logits are, without a gradient of its own.
 static void check(const Tensor& x, const Tensor& t, const char* name, Kind kind, at::IntArrayRef shape) {
     TORCH_CHECK_VALUE(t.defined() && t.device() == x.device(), name, " must be a tensor on ", x.device(), ", where the logits are");
+    no_tangent(t, name);
     TORCH_CHECK_VALUE(!t.requires_grad(), name, " requires grad, but gradients are computed with respect to the logits only: detach it");
     const auto d = t.scalar_type();
     switch (kind) {
@@ -136,6 +143,7 @@ static std::pair<uintptr_t, uintptr_t> span(const Tensor& t) {
 static Tensor check_out(const Tensor& out, const Tensor& x, std::initializer_list<std::pair<const char*, Tensor>> others) {
     TORCH_CHECK_VALUE(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type() && out.device() == x.device(),
                       "out must have the shape, the type and the device of the logits");
+    no_tangent(out, "out");
     TORCH_CHECK_VALUE(!out.is_neg(), "out is a view that torch has yet to negate");
     TORCH_CHECK_VALUE(out.size(-1) == 1 || out.stride(-1) == 1, "the vocabulary must be the contiguous dimension of out");
     int64_t reach = out.size(-1);
@@ -218,6 +226,12 @@ static Scratch scratch(const Tensor& x, at::IntArrayRef rows, int64_t floats) {
     return {at::empty({need + 4 * floats * n_seq * n_tok}, x.options().dtype(at::kByte)), need};
 }
 
+// A gradient that comes into a backward call, or none.
+static Tensor incoming(const Tensor& g) {
+    if (g.defined()) no_tangent(g, "a gradient");
+    return resolved(g);
+}
+
 static bool wants_grad(const Tensor& x) { return at::GradMode::is_enabled() && x.requires_grad(); }
 
 // A gradient that is itself differentiated raises, and not before.
@@ -266,7 +280,7 @@ struct LogprobsNode : torch::autograd::Function<LogprobsNode> {
         return {lp};
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
-        const Tensor g_lp = resolved(g[0]), g_ent = g.size() > 1 ? resolved(g[1]) : Tensor();
+        const Tensor g_lp = incoming(g[0]), g_ent = g.size() > 1 ? incoming(g[1]) : Tensor();
         if (!g_lp.defined() && !g_ent.defined()) return variable_list(2);
         const auto s = ctx->get_saved_variables();
         const Strides none{0, 0};
@@ -362,7 +376,7 @@ struct PolicyNode : torch::autograd::Function<PolicyNode> {
         const float* g_lp = stats + 4 * tokens.numel();
         const Strides dense = row_strides(tokens);
         return {backward_call(x, tokens, s[2], ctx->saved_data["inv_t"].toDouble(), stats, g_lp, dense,
-                              ctx->saved_data["entropy"].toBool() ? g_lp + tokens.numel() : nullptr, dense, resolved(g[0])),
+                              ctx->saved_data["entropy"].toBool() ? g_lp + tokens.numel() : nullptr, dense, incoming(g[0])),
                 Tensor()};
     }
 };
@@ -380,6 +394,12 @@ static Policy3 policy_loss(const Tensor& x, const Tensor& tokens, const Tensor& 
     return {o.loss, o.lp, o.ent};
 }
 
+// The logits of a call that gives their gradient itself.
+static Tensor values_of(const Tensor& x) {
+    no_tangent(x, "logits");      // (detach leaves it behind)
+    return x.detach();
+}
+
 // The version counter of overwritten memory moves, so that autograd notices a use of old values.
 static void overwritten(const OptTensor& out, const Tensor& x) {
     if (!out) return;         // (tensors of inference mode have no counter)
@@ -392,7 +412,7 @@ static std::tuple<Tensor, Tensor, Tensor, Tensor> policy_loss_and_grad(
     double eps_clip, std::optional<double> eps_high, double kl, double ent, double temperature, int reduction, double scale,
     const OptTensor& out) {
     const at::NoGradGuard off;
-    const Tensor x = x_.detach();
+    const Tensor x = values_of(x_);
     const auto p = policy_args(x, tokens, old_lp, adv, mask, ref, eps_clip, eps_high, kl, ent, temperature, reduction, scale);
     const Tensor grad = out ? check_out(*out, x, {{"tokens", p->tokens}, {"mask", p->mask}, {"old_logprobs", p->old_lp},
                                                   {"advantages", p->adv}, {"ref_logprobs", p->ref}})
@@ -455,7 +475,7 @@ struct PreferenceNode : torch::autograd::Function<PreferenceNode> {
         if (!g[0].defined()) return variable_list(2);
         const auto s = ctx->get_saved_variables();
         const float* stats = (const float*)((const char*)s[3].data_ptr() + ctx->saved_data["offset"].toInt());
-        return {backward_call(s[0], s[1], s[2], 1.0, stats, at_of<float>(s[4]), {1, 0}, nullptr, {0, 0}, resolved(g[0])), Tensor()};
+        return {backward_call(s[0], s[1], s[2], 1.0, stats, at_of<float>(s[4]), {1, 0}, nullptr, {0, 0}, incoming(g[0])), Tensor()};
     }
 };
 
@@ -473,7 +493,7 @@ static std::pair<Tensor, Tensor> preference_loss(const Tensor& x, const Tensor& 
 static Policy3 preference_loss_and_grad(const Tensor& x_, const Tensor& tokens, const Tensor& ref, const OptTensor& mask,
                                         double beta, double smoothing, double scale, const OptTensor& out) {
     const at::NoGradGuard off;
-    const Tensor x = x_.detach();
+    const Tensor x = values_of(x_);
     const auto p = preference_args(x, tokens, ref, mask, beta, smoothing, scale);
     const Tensor grad = out ? check_out(*out, x, {{"tokens", p->tokens}, {"mask", p->mask}, {"ref_logprobs", p->ref}}) : grad_like(x);
     const PreferenceOut o = preference_call(x, *p, grad, false);
@@ -540,7 +560,7 @@ struct TeacherNode : torch::autograd::Function<TeacherNode> {
         const Tensor &x = s[0], &index = s[1], &values = s[2];
         const float* stats = (const float*)((const char*)s[4].data_ptr() + ctx->saved_data["offset"].toInt());
         const Call call(x);
-        const Tensor factor = resolved(g[0]), grad = grad_like(x);
+        const Tensor factor = incoming(g[0]), grad = grad_like(x);
         const ppo_token_logits r = rows_of(x, ctx->saved_data["inv_t"].toDouble(), grad);
         done(lib.ppo_distillation_backward(&r, index.data_ptr(), is_i64(index), values.data_ptr(), type_code(values.scalar_type()),
                                            (int)index.size(-1), at_of<uint8_t>(s[3]), stats, at_of<float>(factor), grad.data_ptr(),
@@ -563,7 +583,7 @@ static std::pair<Tensor, Tensor> distillation_loss(const Tensor& x, const Tensor
 static Policy3 distillation_loss_and_grad(const Tensor& x_, const Tensor& index, const Tensor& values, const OptTensor& mask,
                                           double temperature, int reduction, double scale, const OptTensor& out) {
     const at::NoGradGuard off;
-    const Tensor x = x_.detach();
+    const Tensor x = values_of(x_);
     const auto p = teacher_args(x, index, values, mask, temperature, reduction, scale);
     const Tensor grad = out ? check_out(*out, x, {{"teacher_tokens", p->index}, {"teacher_logits", p->logits}, {"mask", p->mask}})
                             : grad_like(x);

@@ -3,8 +3,9 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
-from test_gpu_tokens import K, TYPES, make
+from test_gpu_tokens import K, TYPES, calls, make
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +70,15 @@ def test_lazily_negated_gradients_and_inputs():
     loss = lambda: K().policy_loss(x, y, g_lp - 6, g_h, m)[0]  # noqa: E731
     up = torch.tensor(0.5, device="cuda")
     assert torch.equal(torch.autograd.grad(loss(), x, negated(up))[0], torch.autograd.grad(loss(), x, up)[0])
+
+
+def test_incoming_gradients_with_a_forward_mode_derivative_are_refused():
+    x, y, m = make(24, 2, 3, 500, torch.float32)
+    for fn in calls(x, y, m):
+        a = x.clone().requires_grad_(True)
+        loss = fn(a)
+        with forward_ad.dual_level():
+            up = forward_ad.make_dual(torch.ones_like(loss), torch.ones_like(loss))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(loss, a, up, retain_graph=True)
+        assert torch.isfinite(torch.autograd.grad(loss, a)[0]).all()
