@@ -789,7 +789,7 @@ __device__ __forceinline__ PolicyRow policy_row(const PolicyArgs& p, double lp, 
         const float em1 = expm1f(d);
         o.kl = fabsf(d) < 0.25f
             ? d * d * fmaf(d, fmaf(d, fmaf(d, fmaf(d, fmaf(d, 1.0f / 5040, 1.0f / 720), 1.0f / 120), 1.0f / 24), 1.0f / 6), 0.5f)
-            : em1 - d;
+            : em1 - fminf(d, __FLT_MAX__);     // an impossible token: infinite, not the difference of two infinities
         g = fmaf(-p.kl, em1, g);
     }
     o.g_lp = w * g;

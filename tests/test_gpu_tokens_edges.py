@@ -82,3 +82,19 @@ def test_incoming_gradients_with_a_forward_mode_derivative_are_refused():
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 torch.autograd.grad(loss, a, up, retain_graph=True)
         assert torch.isfinite(torch.autograd.grad(loss, a)[0]).all()
+
+
+@pytest.mark.parametrize("v", [6, 900, 20003, 70001])
+def test_divergence_at_an_impossible_token_is_infinite(v):
+    """ln p = -inf, so d = ref - ln p is +inf and e^d - d - 1 is: not the difference of two infinities."""
+    x, y, _ = make(5, 1, 5, v, torch.float32, masked=False)
+    x[0, 2, y[0, 2]] = -math.inf
+    z = torch.full((1, 5), -2.0, device="cuda")
+    losses = [K().policy_loss_and_grad(x, y, z, z, ref_logprobs=z, kl_coef=0.1)[0],
+              K().policy_loss(x, y, z, z, ref_logprobs=z, kl_coef=0.1)[0]]
+    ref = z.clone()
+    ref[0, 1] = -math.inf                         # a token that the reference policy rules out
+    x[0, 2, y[0, 2]] = 1.0
+    losses.append(K().policy_loss_and_grad(x, y, z, z, ref_logprobs=ref, kl_coef=0.1)[0])
+    for loss in losses:
+        assert float(loss) == math.inf
