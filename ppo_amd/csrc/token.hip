@@ -1204,7 +1204,8 @@ __global__ __launch_bounds__(256) void pair_kernel(const double* __restrict__ lp
             const double z = s[0] - s[1], t = exp(-fabs(z)), l = log1p(t);   // ln(1 + e^-|z|)
             const double neg = (z > 0.0 ? 0.0 : -z) + l, pos = (z > 0.0 ? z : 0.0) + l;   // -ln sig(z), -ln sig(-z); NaN stays in l
             const double sig = z > 0.0 ? 1.0 / (1.0 + t) : t / (1.0 + t);
-            const double loss = scale * ((1.0 - smooth) * neg + (smooth != 0.0 ? smooth * pos : 0.0)) / (double)n_pairs;   // pos may be inf
+            // both may be inf, where the other one alone may count
+            const double loss = scale * ((smooth != 1.0 ? (1.0 - smooth) * neg : 0.0) + (smooth != 0.0 ? smooth * pos : 0.0)) / (double)n_pairs;
             if (solo) *solo = (float)loss;     // the only pair
             else part[q] = loss;
             const float g = (float)(scale * beta * (sig - (1.0 - smooth)) / (double)n_pairs);

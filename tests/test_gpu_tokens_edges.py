@@ -1,4 +1,5 @@
 """GPU tests of the losses over a large vocabulary: layouts and inputs at the edges of what their documentation allows."""
+import ctypes
 import math
 
 import pytest
@@ -98,3 +99,19 @@ def test_divergence_at_an_impossible_token_is_infinite(v):
     losses.append(K().policy_loss_and_grad(x, y, z, z, ref_logprobs=ref, kl_coef=0.1)[0])
     for loss in losses:
         assert float(loss) == math.inf
+
+
+def test_c_abi_pair_of_which_the_label_is_certainly_wrong():
+    """label_smoothing = 1: the rejected sequence is the better one, whatever the preferred one's probability."""
+    from ppo_amd import _lib
+    x, y, _ = make(8, 2, 3, 50, torch.float32, masked=False)
+    x[0, 1, y[0, 1]] = -math.inf                  # the preferred sequence cannot happen: z = -inf, sigmoid(-z) = 1
+    ref, loss, rewards = torch.zeros(2, device="cuda"), torch.ones((), device="cuda"), torch.zeros(2, device="cuda")
+    L = _lib.lib()
+    rows = _lib.TokenLogits(x.data_ptr(), x.stride(0), x.stride(1), 0, 0, 2, 3, 50, 0, 1.0)
+    need = L.ppo_token_workspace_bytes(2, 3)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    code = L.ppo_preference_loss(ctypes.byref(rows), y.data_ptr(), 1, None, ref.data_ptr(), 0.1, 1.0, 1.0, loss.data_ptr(),
+                                 rewards.data_ptr(), None, None, None, ws.data_ptr(), need,
+                                 torch.cuda.current_stream().cuda_stream)
+    assert code == 0 and float(rewards[0]) == -math.inf and float(loss) == 0.0
