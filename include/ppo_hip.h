@@ -321,8 +321,9 @@ int ppo_update_epochs(float* params, int state_dim, int action_dim, int continuo
  *
  * Rows: position t of sequence b of the logits is row r = b * n_tok + t, `vocab` consecutive elements at
  * data + b * seq_stride + t * tok_stride (strides in elements; any values, also 0).  The gradient has the
- * logits' type and strides of its own (no two rows may overlap); it may be the logits' own storage with the
- * same strides, otherwise it must not overlap them.  Arrays "per row" are dense, in row order.
+ * logits' type and strides of its own (no two rows may overlap; the rows of a sequence lie within its stride, or
+ * those of a position within its); it may be the logits' own storage with the same strides, otherwise it must not
+ * overlap them.  Arrays "per row" are dense, in row order.
  * mask (uint8 per row, NULL: all rows count): a row whose entry is 0 does not count.  Its logits, token and
  * other inputs are not used in any way, its outputs are 0 and its row of the gradient is written as zeros.
  * Logits of a counted row may hold -inf (an impossible token); +inf or NaN make its results NaN.  A token

@@ -1529,8 +1529,10 @@ static int check_logits(const ppo_token_logits* x, const void* grad) {
     const uintptr_t size = x->dtype == PPO_F32 ? 4 : 2;
     if (!x->data || (uintptr_t)x->data % size || (uintptr_t)grad % size) return PPO_E_BADARG;
     if (grad) {               // rows of the gradient must not overlap
-        const int64_t s = x->grad_seq_stride, t = x->grad_tok_stride;
-        if ((x->n_tok > 1 && t < x->vocab) || (x->n_seq > 1 && s < (x->n_tok - 1) * t + x->vocab)) return PPO_E_BADARG;
+        // positions within sequences or sequences within positions (a dimension of one row has no stride)
+        const int64_t s = x->n_seq > 1 ? x->grad_seq_stride : INT64_MAX, t = x->n_tok > 1 ? x->grad_tok_stride : INT64_MAX;
+        const int64_t inner = s < t ? s : t, outer = s < t ? t : s, many = s < t ? x->n_seq : x->n_tok;
+        if (inner < x->vocab || (outer != INT64_MAX && (outer - x->vocab) / inner < many - 1)) return PPO_E_BADARG;
     }
     return 0;
 }

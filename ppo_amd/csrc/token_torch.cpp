@@ -146,8 +146,10 @@ static Tensor check_out(const Tensor& out, const Tensor& x, std::initializer_lis
     no_tangent(out, "out");
     TORCH_CHECK_VALUE(!out.is_neg(), "out is a view that torch has yet to negate");
     TORCH_CHECK_VALUE(out.size(-1) == 1 || out.stride(-1) == 1, "the vocabulary must be the contiguous dimension of out");
-    int64_t reach = out.size(-1);
-    for (int64_t d = out.dim() - 2; d >= 0; --d) {
+    int64_t order[2] = {out.dim() - 2, 0}, reach = out.size(-1);     // the rows' dimensions, the closer rows first
+    if (out.dim() == 3 && out.size(0) > 1 && out.size(1) > 1 && out.stride(0) < out.stride(1)) std::swap(order[0], order[1]);
+    for (int64_t k = 0; k < out.dim() - 1; ++k) {
+        const int64_t d = order[k];
         if (out.size(d) <= 1) continue;
         TORCH_CHECK_VALUE(out.stride(d) >= reach, "rows of out overlap");
         reach += (out.size(d) - 1) * out.stride(d);

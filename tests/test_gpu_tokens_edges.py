@@ -6,7 +6,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
-from test_gpu_tokens import K, TYPES, calls, make
+from test_gpu_tokens import K, TYPES, all_three, calls, make
 
 pytestmark = pytest.mark.gpu
 
@@ -41,6 +41,28 @@ def test_a_row_without_entries_has_no_gradient_whatever_its_logits(b, t, v, dtyp
             assert (each[none] == 0).all() and torch.isfinite(each).all()
     for a, c in zip(*results):
         assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype,v", [(torch.float32, 7), (torch.bfloat16, 1001), (torch.float16, 4099), (torch.bfloat16, 70001)])
+def test_gradient_over_logits_of_which_the_tokens_come_first(dtype, v):
+    """Storage [tokens, sequences, vocabulary] seen as [sequences, tokens, vocabulary]: the same bits as in dense memory of
+    the same alignment, in the logits' own place, in other memory of that order and in dense memory."""
+    b, t = 4, 3
+    x, y, m = make(v, b, t, v, dtype)
+    first = torch.zeros(t, b, v + v % 2, dtype=dtype, device="cuda")      # rows on 4-byte boundaries at least
+    view = lambda f: f[..., :v].transpose(0, 1)  # noqa: E731
+    view(first).copy_(x)
+    want = all_three(view(first), y, m)
+    z = torch.full(y.shape, -2.0, device="cuda")
+    index, values = torch.stack([y, (y + 1) % v], -1), torch.stack([z, z - 1], -1)
+    for k, fn in enumerate([lambda a, o: K().policy_loss_and_grad(a, y, z, z, m, ref_logprobs=z, kl_coef=0.1, out=o),
+                            lambda a, o: K().preference_loss_and_grad(a, y, z.sum(-1), m, out=o),
+                            lambda a, o: K().distillation_loss_and_grad(a, index, values, m, out=o)]):
+        own, other = first.clone(), torch.full_like(first, 7.0)
+        for got in (fn(view(own), view(own)), fn(view(first), view(other))):
+            for a, c in zip(want[k], got):
+                assert torch.equal(a, c)
+        assert torch.equal(view(own), want[k][1]) and (other[..., v:] == 7).all()
 
 
 def negated(t):
