@@ -326,8 +326,9 @@ static c10::intrusive_ptr<Policy> policy_args(const Tensor& x, const Tensor& tok
     p->tokens = integers(x, tokens, "tokens", shape);
     p->mask = mask_of(x, mask, shape);
     p->old_lp = floats(x, old_lp, "old_logprobs", shape).contiguous();
-    const bool per_sequence = shape.size() == 2 && adv.sizes() != shape &&
-        ((adv.dim() == 1 && adv.size(0) == shape[0]) || (adv.dim() == 2 && adv.size(0) == shape[0] && adv.size(1) == 1));
+    const int64_t n_seq = shape.size() == 2 ? shape[0] : 1;
+    const bool per_sequence = adv.sizes() != shape &&
+        ((adv.dim() == 1 && adv.size(0) == n_seq) || (adv.dim() == 2 && adv.size(0) == n_seq && adv.size(1) == 1));
     p->adv = floats(x, adv, "advantages", per_sequence ? adv.sizes() : shape);
     p->adv_strides = per_sequence ? Strides{p->adv.stride(0), 0} : row_strides(p->adv);
     TORCH_CHECK_VALUE(ref || kl == 0.0, "kl_coef without ref_logprobs");

@@ -107,6 +107,20 @@ def test_incoming_gradients_with_a_forward_mode_derivative_are_refused():
         assert torch.isfinite(torch.autograd.grad(loss, a)[0]).all()
 
 
+@pytest.mark.parametrize("shape", [(1,), (1, 1)])
+@pytest.mark.parametrize("v", [5, 900, 70001])
+def test_one_advantage_of_the_one_sequence(shape, v):
+    x, y, m = make(9, 1, 7, v, torch.float32)
+    x, y, m = x[0], y[0], torch.arange(7, device="cuda") != 2
+    old, adv = torch.full((7,), -4.0, device="cuda"), torch.full(shape, -1.5, device="cuda")
+    every = adv.reshape(1).expand(7)
+    for a, c in zip(K().policy_loss_and_grad(x, y, old, adv, m), K().policy_loss_and_grad(x, y, old, every, m)):
+        assert torch.equal(a, c)
+    x.requires_grad_(True)
+    a, c = (torch.autograd.grad(K().policy_loss(x, y, old, d, m)[0], x)[0] for d in (adv, every))
+    assert torch.equal(a, c)
+
+
 @pytest.mark.parametrize("v", [6, 900, 20003, 70001])
 def test_divergence_at_an_impossible_token_is_infinite(v):
     """ln p = -inf, so d = ref - ln p is +inf and e^d - d - 1 is: not the difference of two infinities."""

@@ -86,3 +86,14 @@ def test_c_abi_rows_of_the_gradient_in_either_order(n_seq, n_tok, seq, tok, fits
     assert L.ppo_distillation_loss(x, at, 1, at, 0, 4, None, 1, 1.0, at, at, None, at, at, 0, None) == want
     if n_seq % 2 == 0:
         assert L.ppo_preference_loss(x, at, 1, None, at, 0.1, 0.0, 1.0, at, at, None, None, at, at, 0, None) == want
+
+
+@pytest.mark.parametrize("rows,shape,fits", [((3,), (1,), True), ((3,), (1, 1), True), ((3,), (3,), True), ((0,), (1,), True),
+                                             ((3,), (2,), False), ((3,), (3, 1), False), ((3,), (1, 3), False), ((3,), (), False),
+                                             ((2, 3), (2,), True), ((2, 3), (2, 1), True), ((2, 3), (1,), False),
+                                             ((2, 3), (1, 1), False), ((1, 3), (1,), True), ((1, 3), (1, 1), True)])
+def test_shapes_of_advantages(rows, shape, fits):
+    z = torch.zeros(rows)
+    for fn in forms("policy_loss"):
+        with pytest.raises(RuntimeError if fits else ValueError, match="no CPU fallback" if fits else "advantages of shape"):
+            fn(torch.zeros(*rows, 7), z.long(), z, torch.zeros(shape))
