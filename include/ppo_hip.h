@@ -327,7 +327,8 @@ int ppo_update_epochs(float* params, int state_dim, int action_dim, int continuo
  * mask (uint8 per row, NULL: all rows count): a row whose entry is 0 does not count.  Its logits, token and
  * other inputs are not used in any way, its outputs are 0 and its row of the gradient is written as zeros.
  * Logits of a counted row may hold -inf (an impossible token); +inf or NaN make its results NaN.  A token
- * outside [0, vocab) of a counted row makes the row's results and its gradient NaN.
+ * outside [0, vocab) of a counted row makes the row's results and its gradient NaN, but for its entropy, which
+ * does not depend on the token.
  * Sums over the vocabulary and a row's scalars are fp32 and fp64; a gradient is rounded once, to nearest
  * even, to the logits' type.  Results do not depend on other work on the GPU (no atomics).
  * row_stats: 4 floats per row that the forward call leaves for its backward call.

@@ -25,7 +25,8 @@ Common arguments
 
 Logits may be any view whose last dimension is contiguous (``logits[:, :-1]``, a slice of a padded vocabulary).
 Everything runs asynchronously on the current stream of the logits' device; there is no CPU fallback.  A token
-outside the vocabulary makes its row's results NaN.  There are no second and no forward-mode derivatives: both raise.
+outside the vocabulary makes its row's results NaN, but for the entropy, which does not depend on it.  There are no
+second and no forward-mode derivatives: both raise.
 """
 import ctypes
 
