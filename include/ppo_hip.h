@@ -357,8 +357,10 @@ typedef struct {
 size_t ppo_token_workspace_bytes(int64_t n_seq, int64_t n_tok);
 
 /* logprobs[r] of tokens[r] (int32, or int64 with tokens_are_i64) and, where entropy is not NULL, the
- * entropy of the row's distribution.  row_stats may be NULL.  workspace may be NULL: a few long rows then
- * take longer. */
+ * entropy of the row's distribution.  row_stats may be NULL.  workspace may be NULL: a few long rows (at most
+ * PPO_TOKEN_CUT_ROWS of at least PPO_TOKEN_CUT_BYTES; others use none) then take longer. */
+#define PPO_TOKEN_CUT_ROWS 64
+#define PPO_TOKEN_CUT_BYTES 131072
 int ppo_token_logprobs(const ppo_token_logits* x, const void* tokens, int tokens_are_i64, const uint8_t* mask,
                        float* logprobs, float* entropy, float* row_stats, void* workspace,
                        size_t workspace_bytes, void* stream);

@@ -1663,7 +1663,7 @@ static int weights_of(Weights* o, const uint8_t* mask, int reduction, float scal
 static void launch_logprobs(Logits L, int dtype, const void* tokens, int i64, const uint8_t* mask, float* logprobs,
                             double* logprobs64, float* entropy, RowStats* stats, Acc* acc, hipStream_t st) {
     const bool with_e = entropy || logprobs64;
-    if (const int parts = acc ? split_parts(L, dtype, 64, 128 * 1024) : 0) {
+    if (const int parts = acc ? split_parts(L, dtype, PPO_TOKEN_CUT_ROWS, PPO_TOKEN_CUT_BYTES) : 0) {
         const Split sp = {acc, nullptr, parts};
         BY_FLAG(with_e, ENT, {
             BY_TYPE(dtype, T, (split_stats_kernel<T, ENT><<<dim3((unsigned)L.n, parts), 256, 0, st>>>(L, mask, tokens, i64, sp)))

@@ -264,7 +264,7 @@ static std::pair<Tensor, Tensor> logprobs_call(const Tensor& x, const Logprobs& 
     const Call call(x);
     const Tensor lp = new_floats(x, p.tokens.sizes()), ent = p.entropy ? at::empty_like(lp) : Tensor();
     const ppo_token_logits r = rows_of(x, p.inv_t);
-    const bool few_long = p.tokens.numel() <= 64 && x.size(-1) * x.element_size() >= 131072;    // what the library cuts
+    const bool few_long = p.tokens.numel() <= PPO_TOKEN_CUT_ROWS && x.size(-1) * x.element_size() >= PPO_TOKEN_CUT_BYTES;
     const Scratch ws = few_long ? scratch(x, p.tokens.sizes(), 0) : Scratch{Tensor(), 0};
     done(lib.ppo_token_logprobs(&r, p.tokens.data_ptr(), is_i64(p.tokens), at_of<uint8_t>(p.mask), at_of<float>(lp),
                                 at_of<float>(ent), at_of<float>(stats), at_of<void>(ws.memory), (size_t)ws.need, call.stream));
