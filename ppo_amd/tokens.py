@@ -23,7 +23,9 @@ Common arguments
   scale         factor on loss and gradient: the loss scale of float16 training, or 1 / (tokens of all ranks) with
                 reduction="sum" in data-parallel training
 
-Logits may be any view whose last dimension is contiguous (``logits[:, :-1]``, a slice of a padded vocabulary).
+Logits may be any view whose last dimension is contiguous (``logits[:, :-1]``, a slice of a padded vocabulary).  Positions
+that predict nothing may as well be left in and masked off: their rows of the gradient are zeros, and a backward pass has
+no slice to undo.
 Everything runs asynchronously on the current stream of the logits' device; there is no CPU fallback.  A token
 outside the vocabulary makes its row's results NaN, but for the entropy, which does not depend on it.  There are no
 second and no forward-mode derivatives: both raise.
